@@ -1,0 +1,68 @@
+/**
+ * serve_kernels.h - Host-side launchers of the serving operators' kernels
+ * (kernels_attend.hip, kernels_beam.hip), shared by their C entry points
+ * (serving.hip) and the engine. Each checks on the host that the shapes it is
+ * given are those its kernels assume, and returns hipErrorInvalidValue
+ * otherwise, before anything is launched.
+ */
+
+#ifndef SERVE_KERNELS_H
+#define SERVE_KERNELS_H
+
+#include "vitna_hip_internal.h"
+
+#define ATTEND_G_MAX 16 /* query heads a key-value head */
+
+/* A row of the attention, as the caller's vitna_hip_attention_row_t. */
+struct attend_row {
+    int32_t seq, pos, base, shared;
+};
+
+struct attend_args {
+    const void *k, *v; /* element (seq, pos, head, d) at seq * seq_stride + pos * pos_stride + head * head_stride + d */
+    size_t seq_stride, pos_stride, head_stride;
+    int dtype, n_heads, n_kv, hd, ctx, seqs;
+    int window, sinks; /* window 0: none */
+    float scale;       /* of the scores */
+    const float* q;
+    size_t q_stride;
+    float* out;
+    size_t out_stride;
+    int n;
+    /* the rows: n of them in rows, or (rows null) positions run_pos .. run_pos + n - 1 of sequence run_seq */
+    const attend_row* rows;
+    int run_seq, run_pos;
+    /* 1: the rows are tokens of one sequence (a prompt's chunk), rows[i].seq the same for all and nothing shared */
+    int run;
+    int own_max, shared_max; /* the longest own part and the longest shared prefix, about: they size the launch */
+    void* work;
+    size_t work_bytes;
+};
+/* Bytes of work that launch_attend needs for a's shapes (its pointers are not read). */
+size_t attend_work(const attend_args& a);
+hipError_t launch_attend(const attend_args& a, hipStream_t s);
+
+struct beam_select_args {
+    const float* logits;
+    size_t stride, vocab;
+    int groups, width, keep;
+    const float* scores;
+    const uint8_t* ended; /* or null */
+    int end_token;
+    float* best;
+    int *parents, *tokens;
+    void* work;
+};
+size_t beam_select_work(int groups, int width, size_t vocab, int keep);
+hipError_t launch_beam_select(const beam_select_args& a, hipStream_t s);
+
+struct kv_reorder_args {
+    char *k, *v;
+    size_t seq_bytes, layer_bytes, pos_bytes, head_bytes, dim_bytes; /* strides, and a head's bytes */
+    int n_kv, ctx, seqs, layers;
+    const int *list, *parents, *spans;
+    int groups, width, longest;
+};
+hipError_t launch_kv_reorder(const kv_reorder_args& a, hipStream_t s);
+
+#endif

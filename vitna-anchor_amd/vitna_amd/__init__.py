@@ -311,6 +311,13 @@ class RowT(C.Structure):
     _fields_ = [("token", C.c_int32), ("pos", C.c_int32), ("seq", C.c_int32)]
 
 
+class KvView(C.Structure):
+    """vitna_hip_kv_view_t (include/vitna_serve.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int)] + \
+               [(n, C.c_size_t) for n in ("n_heads", "n_kv_heads", "head_dim", "ctx", "seqs", "seq_stride", "pos_stride", "head_stride",
+                                          "window", "sinks")] + [("scale", C.c_float)]
+
+
 def _hip():
     if not os.path.exists(HIP_LIB):
         raise RuntimeError("%s is not built: the HIP path has no fallback. Run python vitna-anchor_amd/build.py" % HIP_LIB)
@@ -378,6 +385,15 @@ def _hip():
         "vitna_hip_copy_probe": (C.c_bool, [C.c_size_t, C.c_int, C.POINTER(C.c_double), *E]),
         "vitna_hip_mfma_probe": (C.c_bool, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double), *E]),
         "vitna_hip_time_steps": (C.c_bool, [P, C.c_size_t, C.c_int32, C.c_size_t, C.c_int, C.POINTER(C.c_double), *E]),
+        "vitna_hip_attention_rows_work": (C.c_size_t, [C.POINTER(KvView), C.c_size_t, C.c_size_t, C.c_size_t]),
+        "vitna_hip_attention_rows": (C.c_bool, [C.POINTER(KvView), P, C.c_size_t, P, C.c_size_t, C.c_size_t, C.c_size_t, P, C.c_size_t, P,
+                                                C.c_size_t, P, *E]),
+        "vitna_hip_attention_run_work": (C.c_size_t, [C.POINTER(KvView), C.c_size_t, C.c_size_t]),
+        "vitna_hip_attention_run": (C.c_bool, [C.POINTER(KvView), C.c_size_t, C.c_size_t, P, C.c_size_t, C.c_size_t, P, C.c_size_t, P,
+                                               C.c_size_t, P, *E]),
+        "vitna_hip_beam_select_work": (C.c_size_t, [C.c_size_t] * 4),
+        "vitna_hip_beam_select": (C.c_bool, [P, *[C.c_size_t] * 5, P, P, C.c_int32, P, P, P, P, C.c_size_t, P, *E]),
+        "vitna_hip_kv_reorder": (C.c_bool, [C.POINTER(KvView), C.c_size_t, C.c_size_t, P, P, P, C.c_size_t, C.c_size_t, C.c_size_t, P, *E]),
         "vitna_hip_time_ffn": (C.c_bool, [P, C.c_int, C.POINTER(C.c_double), *E]),
         "vitna_hip_time_kernel": (C.c_bool, [P, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double),
                                              C.POINTER(C.c_double), *E]),
@@ -767,3 +783,64 @@ def route_check(logits, k, renormalize):
 def matrix_from_bytes(buf, dtype, rows, cols):
     """A Matrix over a numpy byte buffer (kept alive by the caller)."""
     return Matrix(buf.ctypes.data_as(C.c_void_p), dtype, rows, cols)
+
+
+# --- serving operators on device addresses (include/vitna_serve.h); stream: a hipStream_t, 0 the default stream ---
+
+def kv_view(k, v, dtype, n_heads, n_kv_heads, head_dim, ctx, seqs, seq_stride=None, pos_stride=None, head_stride=None, window=0, sinks=0,
+            scale=0.0):
+    """vitna_hip_kv_view_t of a cache at the device addresses k and v. Strides in elements; by default those of
+    [sequence][position][key-value head x dimension]."""
+    head_stride = head_dim if head_stride is None else head_stride
+    pos_stride = n_kv_heads * head_dim if pos_stride is None else pos_stride
+    seq_stride = ctx * pos_stride if seq_stride is None else seq_stride
+    return KvView(k, v, dtype, n_heads, n_kv_heads, head_dim, ctx, seqs, seq_stride, pos_stride, head_stride, window, sinks, scale)
+
+
+def _call(f, *args):
+    err = C.create_string_buffer(512)
+    if not f(*args, err, 512):
+        raise VitnaError(err.value.decode(errors="replace"))
+
+
+def _work(need):
+    if not need:
+        raise VitnaError("the shapes are not served")
+    return need
+
+
+def attention_rows_work(view, n, own_max=0, shared_max=0):
+    """Bytes of work that attention_rows needs for these arguments."""
+    return _work(hip().vitna_hip_attention_rows_work(C.byref(view), n, own_max, shared_max))
+
+
+def attention_rows(view, q, rows, n, out, work, work_bytes, own_max=0, shared_max=0, q_stride=0, out_stride=0, stream=0):
+    """vitna_hip_attention_rows: out = attention of n rows (device int32 n x 4: seq, pos, base, shared) over view's cache."""
+    _call(hip().vitna_hip_attention_rows, view, q, q_stride, rows, n, own_max, shared_max, out, out_stride, work, work_bytes, stream)
+
+
+def attention_run_work(view, pos0, n):
+    """Bytes of work that attention_run needs for these arguments."""
+    return _work(hip().vitna_hip_attention_run_work(C.byref(view), pos0, n))
+
+
+def attention_run(view, seq, pos0, q, n, out, work, work_bytes, q_stride=0, out_stride=0, stream=0):
+    """vitna_hip_attention_run: out = attention of positions pos0 .. pos0 + n - 1 of sequence seq over view's cache."""
+    _call(hip().vitna_hip_attention_run, view, seq, pos0, q, q_stride, n, out, out_stride, work, work_bytes, stream)
+
+
+def beam_select_work(groups, width, vocab, keep):
+    """Bytes of work that beam_select needs for these arguments."""
+    return _work(hip().vitna_hip_beam_select_work(groups, width, vocab, keep))
+
+
+def beam_select(logits, vocab, groups, width, keep, scores, best, parents, tokens, work, work_bytes, ended=0, end_token=0, stride=0,
+                stream=0):
+    """vitna_hip_beam_select: the keep best of each group's width x vocab continuations into best, parents and tokens."""
+    _call(hip().vitna_hip_beam_select, logits, stride, vocab, groups, width, keep, scores, ended, end_token, best, parents, tokens, work,
+          work_bytes, stream)
+
+
+def kv_reorder(view, layers, layer_stride, seqs, parents, spans, groups, width, longest=0, stream=0):
+    """vitna_hip_kv_reorder: each beam's cache from its parent's, in place, in every layer."""
+    _call(hip().vitna_hip_kv_reorder, view, layers, layer_stride, seqs, parents, spans, groups, width, longest, stream)
