@@ -62,7 +62,7 @@ typedef struct {
     if it refuses them. */
 size_t vitna_hip_attention_rows_work(const vitna_hip_kv_view_t* c, size_t n, size_t own_max, size_t shared_max);
 
-/** Attention of n rows (1 <= n <= 65535), each a token of its own: out[i] =
+/** Attention of n rows (1 <= n <= 65535, n x n_kv_heads at most 2^22), each a token of its own: out[i] =
     softmax(scale q[i] k) v over the positions that row i sees, head by head,
     with float32 sums. q and out are n rows of n_heads x head_dim float32,
     q_stride and out_stride floats apart (0: back to back; multiples of 4).
@@ -79,7 +79,8 @@ bool vitna_hip_attention_rows(const vitna_hip_kv_view_t* c, const float* q, size
 /** Bytes of work that vitna_hip_attention_run needs; 0 if it refuses. */
 size_t vitna_hip_attention_run_work(const vitna_hip_kv_view_t* c, size_t pos0, size_t n);
 
-/** The same for n tokens of one sequence (n <= 2^20), at positions pos0 ..
+/** The same for n tokens of one sequence (n <= 2^20, n x n_kv_heads at
+    most 2^22), at positions pos0 ..
     pos0 + n - 1: a prompt's chunk, whose keys and values are in the cache. */
 bool vitna_hip_attention_run(const vitna_hip_kv_view_t* c, size_t seq, size_t pos0, const float* q, size_t q_stride, size_t n, float* out,
                              size_t out_stride, void* work, size_t work_bytes, void* stream, char* err, size_t err_len);
@@ -90,7 +91,7 @@ bool vitna_hip_attention_run(const vitna_hip_kv_view_t* c, size_t seq, size_t po
 size_t vitna_hip_beam_select_work(size_t groups, size_t width, size_t vocab, size_t keep);
 
 /** Beam search's selection: for each of groups prompts with width beams (1 ..
-    VITNA_HIP_BEAMS_MAX), the keep (1 .. VITNA_HIP_BEAMS_MAX) best of its width
+    VITNA_HIP_BEAMS_MAX, at most 2^20 beams in all), the keep (1 .. VITNA_HIP_BEAMS_MAX) best of its width
     x vocab continuations. logits is groups x width rows of vocab float32,
     stride floats apart (0: back to back); scores each beam's sum of log
     probabilities so far. Continuation (b, v) is worth

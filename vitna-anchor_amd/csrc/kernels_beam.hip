@@ -7,100 +7,383 @@
 
 #include <algorithm>
 
-/* ---- selection ---- */
+/* ---- selection ----
+   Two kernels. beam_scan_kernel reads each beam's logits once: a block takes a slice, and leaves the slice's maximum
+   and sum of exponentials and its few logits that can be among the beam's `keep` largest. beam_pick_kernel, a block a
+   group, adds the sums up, gives the candidates their values in 64 bits (two beams' values can lie as near as they
+   like, and which is larger decides) and picks.
 
-/* a row's log of the sum of exponentials, as its maximum and sum */
-__global__ __launch_bounds__(256) void beam_sums_kernel(beam_select_args a) {
-    __shared__ double red[4];
-    __shared__ float redm[4];
-    const int row = blockIdx.x, tid = threadIdx.x;
+   The slice's candidates: every lane's values are four sets, and the keep largest values of a wave's 4096 (or 1024)
+   are at least as large as the keep-th largest of its 256 sets' maxima. That bound is found by halving over the
+   values' order (20 steps of four compares and four counts), the largest of the four waves' bounds holds for the
+   block, and about 1.2 keep values pass it. Where more than BEAM_CAP pass (many equal values) the block picks its
+   keep one by one. */
+
+#define BEAM_WAVES 4
+#define BEAM_CAP 256 /* candidates of a slice at most */
+
+/* float order as unsigned order, no NaN */
+__device__ __forceinline__ uint32_t beam_order(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+}
+
+struct beam_slice {
+    float m, s;  /* maximum, and sum of exp(x - m) */
+    int count;   /* candidates */
+    int pad;
+};
+struct beam_cand {
+    float x;
+    int v;
+};
+
+/* What beam_scan_kernel leaves: slices [rows][splits], candidates [rows][splits][BEAM_CAP]. */
+__host__ __device__ static inline size_t beam_slices_bytes(size_t rows, size_t splits) { return (rows * splits * sizeof(beam_slice) + 255) & ~(size_t)255; }
+
+/* a before b: larger, or equal and of lower index */
+__device__ __forceinline__ bool beam_before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
+
+template <int E, bool VEC>
+__global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_args a, int splits) {
+    __shared__ float sm[BEAM_WAVES], ss[BEAM_WAVES];
+    __shared__ uint32_t st[BEAM_WAVES];
+    __shared__ int sn;
+    const int split = blockIdx.x % splits, row = blockIdx.x / splits, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    beam_slice* slice = static_cast<beam_slice*>(a.work) + (size_t)row * splits + split;
+    if (a.ended && a.ended[row]) return; /* its one continuation needs no logits */
+    beam_cand* cand = reinterpret_cast<beam_cand*>(static_cast<char*>(a.work) + beam_slices_bytes((size_t)a.groups * a.width, splits)) +
+                      ((size_t)row * splits + split) * BEAM_CAP;
     const float* x = a.logits + (size_t)row * a.stride;
-    float m = -INFINITY;
-    for (size_t i = tid; i < a.vocab; i += 256) m = fmaxf(m, x[i]); /* fmaxf passes over NaN */
-    m = wave_max(m);
-    if ((tid & 63) == 0) redm[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
-    double s = 0.0;
-    for (size_t i = tid; i < a.vocab; i += 256) {
-        const float v = x[i];
-        if (v == v && v != -INFINITY) s += v == m ? 1.0 : (double)expf(v - m);
+    const int V = (int)a.vocab, first = (split * BEAM_WAVES + wave) * 64 * E;
+    /* value 4 e + j of a lane: VEC token first + 256 e + 4 lane + j, else first + 64 (4 e + j) + lane */
+    auto token = [&](int e, int j) { return VEC ? first + 256 * e + 4 * lane + j : first + 64 * (4 * e + j) + lane; };
+    float v[E / 4][4];
+#pragma unroll
+    for (int e = 0; e < E / 4; e++) {
+        if (VEC && token(e, 3) < V) {
+            const float4 q = *reinterpret_cast<const float4*>(x + token(e, 0));
+            v[e][0] = q.x; v[e][1] = q.y; v[e][2] = q.z; v[e][3] = q.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[e][j] = token(e, j) < V ? x[token(e, j)] : -INFINITY;
+        }
     }
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, WAVE);
-    if ((tid & 63) == 0) red[tid >> 6] = s;
+    if (tid == 0) sn = 0;
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < E / 4; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[e][j] = fmaxf(v[e][j], -INFINITY); /* a NaN is no continuation */
+            top[j] = fmaxf(top[j], v[e][j]);
+        }
+    const float m = wave_max_dpp(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+    /* sum of exp(x - m): log2(e) in two parts, so that the argument is off by its own rounding alone */
+    float s = 0.0f;
+    if (m > -INFINITY) {
+#pragma unroll
+        for (int e = 0; e < E / 4; e++) {
+            float t[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float d = v[e][j] == m ? 0.0f : v[e][j] - m; /* (infinities) */
+                t[j] = __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f));
+            }
+            s += (t[0] + t[1]) + (t[2] + t[3]);
+        }
+    }
+    s = wave_sum_dpp(s);
+    /* the bound: the largest with at least keep of the wave's 256 maxima at or above it, nearly */
+    uint32_t o[4], lo = 0, hi = beam_order(m);
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = beam_order(top[j]);
+    auto above = [&](uint32_t t) {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) n += __builtin_popcountll(__ballot(o[j] >= t));
+        return n;
+    };
+    {
+        /* from the smallest of the lanes' maxima, which 64 of them reach */
+        uint32_t least = ~max(max(o[0], o[1]), max(o[2], o[3]));
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) least = max(least, (uint32_t)__shfl_xor((int)least, d, WAVE));
+        lo = ~least;
+        for (int step = 0; step < 20 && lo < hi; step++) {
+            const uint32_t mid = lo + (hi - lo) / 2 + 1;
+            const int n = above(mid);
+            if (n >= a.keep) {
+                lo = mid;
+                if (n == a.keep) break;
+            } else {
+                hi = mid - 1;
+            }
+        }
+    }
+    if (lane == 0) {
+        sm[wave] = m;
+        ss[wave] = s;
+        st[wave] = lo;
+    }
     __syncthreads();
+    lo = max(max(max(st[0], st[1]), max(st[2], st[3])), beam_order(-INFINITY) + 1);
+#pragma unroll
+    for (int e = 0; e < E / 4; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (beam_order(v[e][j]) >= lo) {
+                const int at = atomicAdd(&sn, 1); /* in any order: the values decide later */
+                if (at < BEAM_CAP) cand[at] = beam_cand{v[e][j], token(e, j)};
+            }
+    __syncthreads();
+    const int n = sn;
+    if (n > BEAM_CAP) {
+        /* many alike: the keep first of them, one a round, by value and then by index */
+        __shared__ float rx[BEAM_WAVES];
+        __shared__ int ri[BEAM_WAVES];
+        float lx = INFINITY;
+        int li = -1;
+        for (int round = 0; round < a.keep; round++) {
+            float bx = -INFINITY;
+            int bi = INT32_MAX;
+#pragma unroll
+            for (int e = 0; e < E / 4; e++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float y = v[e][j];
+                    const int i = token(e, j);
+                    if (y > -INFINITY && beam_before(lx, li, y, i) && beam_before(y, i, bx, bi)) { bx = y; bi = i; }
+                }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const float y = __shfl_xor(bx, d, WAVE);
+                const int i = __shfl_xor(bi, d, WAVE);
+                if (beam_before(y, i, bx, bi)) { bx = y; bi = i; }
+            }
+            if (lane == 0) { rx[wave] = bx; ri[wave] = bi; }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < BEAM_WAVES; w++)
+                if (beam_before(rx[w], ri[w], bx, bi)) { bx = rx[w]; bi = ri[w]; }
+            __syncthreads();
+            if (tid == 0) cand[round] = beam_cand{bx, bi};
+            lx = bx;
+            li = bi;
+        }
+    }
     if (tid == 0) {
-        double* out = (double*)a.work + 2 * (size_t)row;
-        out[0] = (double)m;
-        out[1] = log((red[0] + red[1]) + (red[2] + red[3]));
+        float M = -INFINITY, S = 0.0f;
+        for (int w = 0; w < BEAM_WAVES; w++) M = fmaxf(M, sm[w]);
+        for (int w = 0; w < BEAM_WAVES; w++)
+            if (ss[w] > 0.0f) S += ss[w] * (sm[w] == M ? 1.0f : expf(sm[w] - M));
+        *slice = beam_slice{M, S, n > BEAM_CAP ? a.keep : n, 0};
     }
 }
 
-__device__ __forceinline__ bool beam_better(double v, int64_t i, double w, int64_t j) { return v > w || (v == w && i < j); }
+#define PICK_THREADS 1024
+#define PICK_BINS 2048
+#define PICK_CAP 512 /* continuations that are ranked by counting */
 
-/* one round a result: the best continuation behind the last one in the order */
-__global__ __launch_bounds__(256) void beam_rounds_kernel(beam_select_args a) {
-    __shared__ double rv[4];
-    __shared__ int64_t ri[4];
-    const int group = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_args a, int splits) {
+    __shared__ double s_score[64], s_log[64]; /* of a beam: its score, log of its sum of exponentials */
+    __shared__ float s_most[64];              /* and its largest logit */
+    __shared__ int s_hist[PICK_BINS], s_wave[PICK_THREADS / 64], s_found[2], s_n;
+    __shared__ double r_v[PICK_THREADS / 64];
+    __shared__ int64_t r_i[PICK_THREADS / 64];
+    __shared__ double c_v[PICK_CAP];
+    __shared__ int64_t c_i[PICK_CAP];
+    const int group = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, W = a.width;
+    const beam_slice* slices = static_cast<const beam_slice*>(a.work) + (size_t)group * W * splits;
+    const beam_cand* cands = reinterpret_cast<const beam_cand*>(static_cast<const char*>(a.work) + beam_slices_bytes((size_t)a.groups * W, splits)) +
+                             (size_t)group * W * splits * BEAM_CAP;
     const int64_t V = (int64_t)a.vocab;
-    double last = INFINITY;
-    int64_t last_at = -1;
-    for (int round = 0; round < a.keep; round++) {
-        double bv = -INFINITY;
-        int64_t bi = INT64_MAX;
-        for (int b = 0; b < a.width; b++) {
-            const int row = group * a.width + b;
-            const double score = (double)a.scores[row], m = ((double*)a.work)[2 * (size_t)row], l = ((double*)a.work)[2 * (size_t)row + 1];
-            if (!(score > -INFINITY)) continue;
-            const bool ended = a.ended && a.ended[row];
-            for (int64_t i = tid; i < V; i += 256) {
-                double v;
-                if (ended) {
-                    if (i != a.end_token) continue;
-                    v = score;
-                } else {
-                    const double x = (double)a.logits[(size_t)row * a.stride + i];
-                    if (!(x > -INFINITY)) continue;
-                    v = score + ((x == m ? 0.0 : x - m) - l);
-                    if (!(v > -INFINITY)) continue;
-                }
-                const int64_t at = b * V + i;
-                if (beam_better(v, at, bv, bi) && beam_better(last, last_at, v, at)) { bv = v; bi = at; }
+    for (int b = wave; b < W; b += PICK_THREADS / 64) {
+        const int row = group * W + b;
+        const float score = a.scores[row];
+        const bool dead = !(score > -INFINITY), ended = a.ended && a.ended[row];
+        float m = -INFINITY;
+        double s = 0.0;
+        if (!ended) {
+            for (int i = lane; i < splits; i += 64) m = fmaxf(m, slices[b * splits + i].m);
+            m = wave_max_dpp(m);
+            for (int i = lane; i < splits; i += 64) {
+                const beam_slice t = slices[b * splits + i];
+                if (t.s > 0.0f) s += (double)t.s * (t.m == m ? 1.0 : exp((double)t.m - (double)m));
+            }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, WAVE);
+        }
+        if (lane == 0) {
+            s_score[b] = dead ? -INFINITY : (double)score;
+            s_most[b] = m;
+            s_log[b] = ended ? 0.0 : log(s);
+        }
+    }
+    __syncthreads();
+    /* every continuation left, to f(value, index): a wave a slice, and a thread a beam that ended */
+    auto each = [&](auto f) {
+        for (int i = wave; i < W * splits; i += PICK_THREADS / 64) {
+            const int b = i / splits;
+            const double score = s_score[b];
+            if (!(score > -INFINITY) || (a.ended && a.ended[group * W + b])) continue;
+            const int n = slices[i].count;
+            const float m = s_most[b];
+            for (int c = lane; c < n; c += 64) {
+                const beam_cand t = cands[(size_t)i * BEAM_CAP + c];
+                const double v = score + ((t.x == m ? 0.0 : (double)t.x - (double)m) - s_log[b]);
+                if (v > -INFINITY) f(v, (int64_t)b * V + t.v);
             }
         }
-        for (int o = 32; o > 0; o >>= 1) {
-            const double ov = __shfl_xor(bv, o, WAVE);
-            const int64_t oi = __shfl_xor(bi, o, WAVE);
-            if (beam_better(ov, oi, bv, bi)) { bv = ov; bi = oi; }
-        }
-        __syncthreads();
-        if ((tid & 63) == 0) { rv[tid >> 6] = bv; ri[tid >> 6] = bi; }
-        __syncthreads();
-        for (int w = 0; w < 4; w++)
-            if (beam_better(rv[w], ri[w], bv, bi)) { bv = rv[w]; bi = ri[w]; }
-        const bool none = bi == INT64_MAX;
-        if (tid == 0) {
-            const int at = group * a.keep + round;
-            a.best[at] = none ? -INFINITY : (float)bv;
-            a.parents[at] = none ? -1 : (int)(bi / V);
-            a.tokens[at] = none ? -1 : (int)(bi % V);
-        }
-        last = bv;
-        last_at = bi;
+        if (a.ended && tid < W && a.ended[group * W + tid] && s_score[tid] > -INFINITY) f(s_score[tid], (int64_t)tid * V + a.end_token);
+    };
+    /* the range of the values, and how many there are */
+    double most = -INFINITY, least = INFINITY;
+    int mine = 0;
+    each([&](double v, int64_t) {
+        most = fmax(most, v);
+        least = fmin(least, v);
+        mine++;
+    });
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        most = fmax(most, __shfl_xor(most, d, WAVE));
+        least = fmin(least, __shfl_xor(least, d, WAVE));
+        mine += __shfl_xor(mine, d, WAVE);
     }
+    if (lane == 0) { r_v[wave] = most; r_i[wave] = __double_as_longlong(least); s_wave[wave] = mine; }
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < PICK_THREADS / 64; w++) {
+        most = fmax(most, r_v[w]);
+        least = fmin(least, __longlong_as_double(r_i[w]));
+        total += s_wave[w];
+    }
+    const int keep = min(a.keep, total);
+    /* t(v) = how far v lies below the largest, 0 .. PICK_BINS of the range: those with t < from + width are kept, and
+       the bin that holds the keep-th is cut again until they are few */
+    const double scale = most > least && most < INFINITY ? PICK_BINS / (most - least) : 0.0;
+    auto below = [&](double v) { return v == most ? 0.0 : (most - v) * scale; };
+    double from = 0.0, width = PICK_BINS + 1.0;
+    int before = 0, kept = total;
+    for (int level = 0; level < 5 && kept > PICK_CAP; level++) {
+        const double bins = PICK_BINS / width;
+        for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_hist[i] = 0;
+        if (tid == 0) { s_found[0] = 0; s_found[1] = before; s_n = kept; }
+        __syncthreads();
+        each([&](double v, int64_t) {
+            const double t = (below(v) - from) * bins;
+            if (t >= 0.0 && t < PICK_BINS) atomicAdd(&s_hist[(int)t], 1);
+        });
+        __syncthreads();
+        /* two bins a thread: the bin where before + the counts so far reaches keep */
+        const int h0 = s_hist[2 * tid], h1 = s_hist[2 * tid + 1];
+        int run = h0 + h1;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(run, d, WAVE);
+            if (lane >= d) run += o;
+        }
+        if (lane == 63) s_wave[wave] = run;
+        __syncthreads();
+        int at = before;
+        for (int w = 0; w < wave; w++) at += s_wave[w];
+        const int b0 = at + run - h0 - h1, b1 = b0 + h0, b2 = b1 + h1; /* before bin 2 tid, before 2 tid + 1, behind it */
+        if (b0 < keep && b1 >= keep) { s_found[0] = 2 * tid; s_found[1] = b0; s_n = b1; }
+        if (b1 < keep && b2 >= keep) { s_found[0] = 2 * tid + 1; s_found[1] = b1; s_n = b2; }
+        __syncthreads();
+        from += s_found[0] / bins;
+        width /= PICK_BINS;
+        before = s_found[1];
+        kept = s_n;
+        __syncthreads();
+    }
+    float* best = a.best + (size_t)group * a.keep;
+    int *parents = a.parents + (size_t)group * a.keep, *tokens = a.tokens + (size_t)group * a.keep;
+    auto put = [&](int at, double v, int64_t i) {
+        best[at] = (float)v;
+        parents[at] = (int)(i / V);
+        tokens[at] = (int)(i % V);
+    };
+    for (int i = keep + tid; i < a.keep; i += PICK_THREADS) {
+        best[i] = -INFINITY;
+        parents[i] = -1;
+        tokens[i] = -1;
+    }
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    if (kept <= PICK_CAP) {
+        each([&](double v, int64_t i) {
+            if (below(v) < from + width) {
+                const int at = atomicAdd(&s_n, 1);
+                if (at < PICK_CAP) { c_v[at] = v; c_i[at] = i; }
+            }
+        });
+        __syncthreads();
+    }
+    const int n = s_n;
+    if (kept <= PICK_CAP && n <= PICK_CAP && n >= keep) {
+        if (tid < n) {
+            const double v = c_v[tid];
+            const int64_t i = c_i[tid];
+            int rank = 0;
+            for (int j = 0; j < n && rank < keep; j++) rank += c_v[j] > v || (c_v[j] == v && c_i[j] < i);
+            if (rank < keep) put(rank, v, i);
+        }
+        return;
+    }
+    /* more alike than can be ranked so: one a round */
+    double last = INFINITY;
+    int64_t last_i = -1;
+    for (int round = 0; round < keep; round++) {
+        double bv = -INFINITY;
+        int64_t bi = INT64_MAX;
+        each([&](double v, int64_t i) {
+            if ((v < last || (v == last && i > last_i)) && (v > bv || (v == bv && i < bi))) { bv = v; bi = i; }
+        });
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double v = __shfl_xor(bv, d, WAVE);
+            const int64_t i = __shfl_xor(bi, d, WAVE);
+            if (v > bv || (v == bv && i < bi)) { bv = v; bi = i; }
+        }
+        __syncthreads();
+        if (lane == 0) { r_v[wave] = bv; r_i[wave] = bi; }
+        __syncthreads();
+        for (int w = 0; w < PICK_THREADS / 64; w++)
+            if (r_v[w] > bv || (r_v[w] == bv && r_i[w] < bi)) { bv = r_v[w]; bi = r_i[w]; }
+        if (tid == 0) put(round, bv, bi);
+        last = bv;
+        last_i = bi;
+    }
+}
+
+/* Values a lane of the scan: 64 where that leaves two blocks a compute unit, else 16. */
+static int beam_lane_values(int rows, size_t vocab) { return (size_t)rows * vocab >= (size_t)512 * BEAM_WAVES * 64 * 64 ? 64 : 16; }
+static int beam_splits(int rows, size_t vocab) {
+    const size_t slice = (size_t)BEAM_WAVES * 64 * beam_lane_values(rows, vocab);
+    return (int)((vocab + slice - 1) / slice);
 }
 
 size_t beam_select_work(int groups, int width, size_t vocab, int keep) {
-    (void)vocab;
     (void)keep;
-    return (size_t)groups * width * 16;
+    const size_t rows = (size_t)groups * width, splits = beam_splits((int)rows, vocab);
+    return beam_slices_bytes(rows, splits) + rows * splits * BEAM_CAP * sizeof(beam_cand);
 }
 
 hipError_t launch_beam_select(const beam_select_args& a, hipStream_t s) {
-    if (a.groups < 1 || a.width < 1 || a.keep < 1) return hipErrorInvalidValue;
-    beam_sums_kernel<<<a.groups * a.width, 256, 0, s>>>(a);
-    beam_rounds_kernel<<<a.groups, 256, 0, s>>>(a);
+    if (a.groups < 1 || a.width < 1 || a.width > 64 || a.keep < 1 || a.keep > 64) return hipErrorInvalidValue;
+    const int rows = a.groups * a.width, splits = beam_splits(rows, a.vocab), E = beam_lane_values(rows, a.vocab);
+    if ((size_t)rows * splits > ((size_t)1 << 23)) return hipErrorInvalidValue; /* threads of a launch stay within 32 bits */
+    const int grid = rows * splits;
+    const bool vec = ((uintptr_t)a.logits & 15) == 0 && a.stride % 4 == 0;
+    if (E == 64) {
+        if (vec) beam_scan_kernel<64, true><<<grid, 64 * BEAM_WAVES, 0, s>>>(a, splits);
+        else beam_scan_kernel<64, false><<<grid, 64 * BEAM_WAVES, 0, s>>>(a, splits);
+    } else {
+        if (vec) beam_scan_kernel<16, true><<<grid, 64 * BEAM_WAVES, 0, s>>>(a, splits);
+        else beam_scan_kernel<16, false><<<grid, 64 * BEAM_WAVES, 0, s>>>(a, splits);
+    }
+    beam_pick_kernel<<<a.groups, PICK_THREADS, 0, s>>>(a, splits);
     return hipGetLastError();
 }
 

@@ -105,6 +105,8 @@ static bool attend_shape(const vitna_hip_kv_view_t* c, size_t n, attend_args* a,
     if (!check_view(c, err, err_len)) return false;
     if (c->n_heads < 1 || c->n_heads % c->n_kv_heads || c->n_heads / c->n_kv_heads > ATTEND_G_MAX)
         return fail(err, err_len, "%zu query heads of %zu key-value heads; 1 to %d of each are served", c->n_heads, c->n_kv_heads, ATTEND_G_MAX);
+    /* the launches' threads stay within 32 bits */
+    if (n * c->n_kv_heads > ((size_t)1 << 22)) return fail(err, err_len, "%zu rows of %zu key-value heads; %d of both are served", n, c->n_kv_heads, 1 << 22);
     if (!(c->scale >= 0.0f) || c->scale > 3e38f) return fail(err, err_len, "a scale of %g; 0 or a positive number is needed", (double)c->scale);
     *a = attend_args();
     a->k = c->k; a->v = c->v;
@@ -188,6 +190,7 @@ static bool select_shape(size_t groups, size_t width, size_t vocab, size_t keep,
     if (groups < 1 || groups > 65535) return fail(err, err_len, "%zu groups; 1 to 65535 are served", groups);
     if (width < 1 || width > VITNA_HIP_BEAMS_MAX) return fail(err, err_len, "%zu beams; 1 to %d are served", width, VITNA_HIP_BEAMS_MAX);
     if (keep < 1 || keep > VITNA_HIP_BEAMS_MAX) return fail(err, err_len, "%zu results; 1 to %d are served", keep, VITNA_HIP_BEAMS_MAX);
+    if (groups * width > ((size_t)1 << 20)) return fail(err, err_len, "%zu groups of %zu beams; %d beams in all are served", groups, width, 1 << 20);
     if (vocab < 1 || vocab > ((size_t)1 << 24)) return fail(err, err_len, "a vocabulary of %zu; 1 to %d are served", vocab, 1 << 24);
     return true;
 }
