@@ -8,19 +8,19 @@
 #include <algorithm>
 
 /* ---- selection ----
-   Two kernels. beam_scan_kernel reads each beam's logits once: a block takes a slice, and leaves the slice's maximum
-   and sum of exponentials and its few logits that can be among the beam's `keep` largest. beam_pick_kernel, a block a
-   group, adds the sums up, gives the candidates their values in 64 bits (two beams' values can lie as near as they
-   like, and which is larger decides) and picks.
+   Two kernels. beam_scan_kernel reads each beam's logits once: a block takes a slice, and leaves the slice's maximum,
+   its sum of exponentials and its `keep` largest logits in order. beam_pick_kernel, a block a group, adds the sums
+   up, gives those logits their values in 64 bits (two beams' values can lie as near as they like, and which is larger
+   decides) and ranks the ones that can be among the group's `keep` best.
 
-   The slice's candidates: every lane's values are four sets, and the keep largest values of a wave's 4096 (or 1024)
-   are at least as large as the keep-th largest of its 256 sets' maxima. That bound is found by halving over the
-   values' order (20 steps of four compares and four counts), the largest of the four waves' bounds holds for the
-   block, and about 1.2 keep values pass it. Where more than BEAM_CAP pass (many equal values) the block picks its
-   keep one by one. */
+   The slice's largest: every lane's values are four sets, and the keep largest values of a wave's 4096 (or 1024) are
+   at least as large as the keep-th largest of its 256 sets' maxima. That bound is found by halving over the values'
+   order (20 steps of four compares and four counts), the largest of the four waves' bounds holds for the block, and
+   one and a half to four times keep values pass it: each counts those before it. Where more than BEAM_CAP pass (many
+   equal values) the block picks its keep one by one. */
 
 #define BEAM_WAVES 4
-#define BEAM_CAP 256 /* candidates of a slice at most */
+#define BEAM_CAP 512
 
 /* float order as unsigned order, no NaN */
 __device__ __forceinline__ uint32_t beam_order(float x) {
@@ -28,20 +28,15 @@ __device__ __forceinline__ uint32_t beam_order(float x) {
     return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-struct beam_slice {
-    float m, s;  /* maximum, and sum of exp(x - m) */
-    int count;   /* candidates */
-    int pad;
-};
 struct beam_cand {
-    float x;
-    int v;
+    float x; /* a logit, -inf: none */
+    int v;   /* its token */
 };
 
-/* What beam_scan_kernel leaves: slices [rows][splits], candidates [rows][splits][BEAM_CAP]. */
-__host__ __device__ static inline size_t beam_slices_bytes(size_t rows, size_t splits) { return (rows * splits * sizeof(beam_slice) + 255) & ~(size_t)255; }
+/* What beam_scan_kernel leaves: (maximum, sum) of [rows][splits], then beam_cand of [rows][splits][keep]. */
+static __host__ __device__ size_t beam_sums_bytes(size_t slices) { return (slices * sizeof(float2) + 255) & ~(size_t)255; }
 
-/* a before b: larger, or equal and of lower index */
+/* x at i comes before y at j: larger, or equal and of lower index */
 __device__ __forceinline__ bool beam_before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
 template <int E, bool VEC>
@@ -49,11 +44,11 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
     __shared__ float sm[BEAM_WAVES], ss[BEAM_WAVES];
     __shared__ uint32_t st[BEAM_WAVES];
     __shared__ int sn;
+    __shared__ beam_cand sc[BEAM_CAP];
     const int split = blockIdx.x % splits, row = blockIdx.x / splits, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    beam_slice* slice = static_cast<beam_slice*>(a.work) + (size_t)row * splits + split;
     if (a.ended && a.ended[row]) return; /* its one continuation needs no logits */
-    beam_cand* cand = reinterpret_cast<beam_cand*>(static_cast<char*>(a.work) + beam_slices_bytes((size_t)a.groups * a.width, splits)) +
-                      ((size_t)row * splits + split) * BEAM_CAP;
+    beam_cand* out = reinterpret_cast<beam_cand*>(static_cast<char*>(a.work) + beam_sums_bytes((size_t)a.groups * a.width * splits)) +
+                     (size_t)blockIdx.x * a.keep;
     const float* x = a.logits + (size_t)row * a.stride;
     const int V = (int)a.vocab, first = (split * BEAM_WAVES + wave) * 64 * E;
     /* value 4 e + j of a lane: VEC token first + 256 e + 4 lane + j, else first + 64 (4 e + j) + lane */
@@ -95,7 +90,7 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
     }
     s = wave_sum_dpp(s);
     /* the bound: the largest with at least keep of the wave's 256 maxima at or above it, nearly */
-    uint32_t o[4], lo = 0, hi = beam_order(m);
+    uint32_t o[4], lo, hi = beam_order(m);
 #pragma unroll
     for (int j = 0; j < 4; j++) o[j] = beam_order(top[j]);
     auto above = [&](uint32_t t) {
@@ -128,144 +123,215 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
     }
     __syncthreads();
     lo = max(max(max(st[0], st[1]), max(st[2], st[3])), beam_order(-INFINITY) + 1);
-#pragma unroll
-    for (int e = 0; e < E / 4; e++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (beam_order(v[e][j]) >= lo) {
-                const int at = atomicAdd(&sn, 1); /* in any order: the values decide later */
-                if (at < BEAM_CAP) cand[at] = beam_cand{v[e][j], token(e, j)};
-            }
-    __syncthreads();
-    const int n = sn;
-    if (n > BEAM_CAP) {
-        /* many alike: the keep first of them, one a round, by value and then by index */
-        __shared__ float rx[BEAM_WAVES];
-        __shared__ int ri[BEAM_WAVES];
-        float lx = INFINITY;
-        int li = -1;
-        for (int round = 0; round < a.keep; round++) {
-            float bx = -INFINITY;
-            int bi = INT32_MAX;
-#pragma unroll
-            for (int e = 0; e < E / 4; e++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float y = v[e][j];
-                    const int i = token(e, j);
-                    if (y > -INFINITY && beam_before(lx, li, y, i) && beam_before(y, i, bx, bi)) { bx = y; bi = i; }
-                }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const float y = __shfl_xor(bx, d, WAVE);
-                const int i = __shfl_xor(bi, d, WAVE);
-                if (beam_before(y, i, bx, bi)) { bx = y; bi = i; }
-            }
-            if (lane == 0) { rx[wave] = bx; ri[wave] = bi; }
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < BEAM_WAVES; w++)
-                if (beam_before(rx[w], ri[w], bx, bi)) { bx = rx[w]; bi = ri[w]; }
-            __syncthreads();
-            if (tid == 0) cand[round] = beam_cand{bx, bi};
-            lx = bx;
-            li = bi;
-        }
-    }
     if (tid == 0) {
         float M = -INFINITY, S = 0.0f;
         for (int w = 0; w < BEAM_WAVES; w++) M = fmaxf(M, sm[w]);
         for (int w = 0; w < BEAM_WAVES; w++)
             if (ss[w] > 0.0f) S += ss[w] * (sm[w] == M ? 1.0f : expf(sm[w] - M));
-        *slice = beam_slice{M, S, n > BEAM_CAP ? a.keep : n, 0};
+        static_cast<float2*>(a.work)[blockIdx.x] = make_float2(M, S);
+    }
+#pragma unroll
+    for (int e = 0; e < E / 4; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (beam_order(v[e][j]) >= lo) {
+                const int at = atomicAdd(&sn, 1); /* in any order: they are ranked */
+                if (at < BEAM_CAP) sc[at] = beam_cand{v[e][j], token(e, j)};
+            }
+    __syncthreads();
+    const int n = sn;
+    for (int i = n + tid; i < a.keep; i += 64 * BEAM_WAVES) out[i] = beam_cand{-INFINITY, INT32_MAX};
+    if (n <= BEAM_CAP) {
+        for (int i = tid; i < n; i += 64 * BEAM_WAVES) {
+            const beam_cand mine = sc[i];
+            int rank = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; j++) rank += beam_before(sc[j].x, sc[j].v, mine.x, mine.v);
+            if (rank < a.keep) out[rank] = mine;
+        }
+        return;
+    }
+    /* many alike: the keep first of them, one a round */
+    __shared__ float rx[BEAM_WAVES];
+    __shared__ int ri[BEAM_WAVES];
+    float lx = INFINITY;
+    int li = -1;
+    for (int round = 0; round < a.keep; round++) {
+        float bx = -INFINITY;
+        int bi = INT32_MAX;
+#pragma unroll
+        for (int e = 0; e < E / 4; e++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float y = v[e][j];
+                const int i = token(e, j);
+                if (y > -INFINITY && beam_before(lx, li, y, i) && beam_before(y, i, bx, bi)) { bx = y; bi = i; }
+            }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const float y = __shfl_xor(bx, d, WAVE);
+            const int i = __shfl_xor(bi, d, WAVE);
+            if (beam_before(y, i, bx, bi)) { bx = y; bi = i; }
+        }
+        if (lane == 0) { rx[wave] = bx; ri[wave] = bi; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < BEAM_WAVES; w++)
+            if (beam_before(rx[w], ri[w], bx, bi)) { bx = rx[w]; bi = ri[w]; }
+        __syncthreads();
+        if (tid == 0) out[round] = beam_cand{bx, bi};
+        lx = bx;
+        li = bi;
     }
 }
 
 #define PICK_THREADS 1024
+#define PICK_WAVES (PICK_THREADS / 64)
+#define PICK_HELD 8    /* candidates a thread asks for before anything else, and holds */
 #define PICK_BINS 2048
-#define PICK_CAP 512 /* continuations that are ranked by counting */
+#define PICK_CAP 512   /* continuations that are ranked by counting */
 
 __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_args a, int splits) {
-    __shared__ double s_score[64], s_log[64]; /* of a beam: its score, log of its sum of exponentials */
-    __shared__ float s_most[64];              /* and its largest logit */
-    __shared__ int s_hist[PICK_BINS], s_wave[PICK_THREADS / 64], s_found[2], s_n;
-    __shared__ double r_v[PICK_THREADS / 64];
-    __shared__ int64_t r_i[PICK_THREADS / 64];
+    __shared__ double s_score[64], s_log[64]; /* of a beam: its score (-inf: it has no continuations), log of its sum of exponentials */
+    __shared__ double s_bound[64];            /* keep of its continuations are worth this or more */
+    __shared__ float s_most[64];              /* its largest logit */
+    __shared__ int s_hist[PICK_BINS], s_wave[PICK_WAVES], s_found[2], s_n;
+    __shared__ double r_v[PICK_WAVES];
+    __shared__ int64_t r_i[PICK_WAVES];
     __shared__ double c_v[PICK_CAP];
     __shared__ int64_t c_i[PICK_CAP];
-    const int group = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, W = a.width;
-    const beam_slice* slices = static_cast<const beam_slice*>(a.work) + (size_t)group * W * splits;
-    const beam_cand* cands = reinterpret_cast<const beam_cand*>(static_cast<const char*>(a.work) + beam_slices_bytes((size_t)a.groups * W, splits)) +
-                             (size_t)group * W * splits * BEAM_CAP;
+    const int group = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, W = a.width, K = a.keep;
+    const size_t slices = (size_t)a.groups * W * splits;
+    const float2* sums = static_cast<const float2*>(a.work) + (size_t)group * W * splits;
+    const beam_cand* cands = reinterpret_cast<const beam_cand*>(static_cast<const char*>(a.work) + beam_sums_bytes(slices)) + (size_t)group * W * splits * K;
     const int64_t V = (int64_t)a.vocab;
-    for (int b = wave; b < W; b += PICK_THREADS / 64) {
+    const int row_cands = splits * K, total = W * row_cands;
+    beam_cand held[PICK_HELD];
+#pragma unroll
+    for (int r = 0; r < PICK_HELD; r++)
+        if (tid + PICK_THREADS * r < total) held[r] = cands[tid + PICK_THREADS * r];
+    for (int b = wave; b < W; b += PICK_WAVES) {
         const int row = group * W + b;
         const float score = a.scores[row];
-        const bool dead = !(score > -INFINITY), ended = a.ended && a.ended[row];
-        float m = -INFINITY;
-        double s = 0.0;
-        if (!ended) {
-            for (int i = lane; i < splits; i += 64) m = fmaxf(m, slices[b * splits + i].m);
-            m = wave_max_dpp(m);
-            for (int i = lane; i < splits; i += 64) {
-                const beam_slice t = slices[b * splits + i];
-                if (t.s > 0.0f) s += (double)t.s * (t.m == m ? 1.0 : exp((double)t.m - (double)m));
-            }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, WAVE);
+        const bool ended = a.ended && a.ended[row];
+        float2 t = make_float2(-INFINITY, 0.0f);
+        float bound = -INFINITY;
+        if (lane < splits) {
+            t = sums[b * splits + lane];
+            bound = cands[(b * splits + lane) * K + K - 1].x;
         }
+        float m = t.x;
+        for (int i = lane + 64; i < splits; i += 64) {
+            m = fmaxf(m, sums[b * splits + i].x);
+            bound = fmaxf(bound, cands[(b * splits + i) * K + K - 1].x);
+        }
+        m = wave_max_dpp(m);
+        bound = wave_max_dpp(bound);
+        double s = t.y > 0.0f ? (double)(t.y * (t.x == m ? 1.0f : expf(t.x - m))) : 0.0;
+        for (int i = lane + 64; i < splits; i += 64) {
+            const float2 u = sums[b * splits + i];
+            if (u.y > 0.0f) s += (double)(u.y * (u.x == m ? 1.0f : expf(u.x - m)));
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, WAVE);
         if (lane == 0) {
-            s_score[b] = dead ? -INFINITY : (double)score;
+            const double l = log(s);
+            const bool on = score > -INFINITY && !ended; /* an ended beam's slices hold nothing */
+            s_score[b] = on ? (double)score : -INFINITY;
             s_most[b] = m;
-            s_log[b] = ended ? 0.0 : log(s);
+            s_log[b] = l;
+            s_bound[b] = on && bound > -INFINITY ? (double)score + ((bound == m ? 0.0 : (double)bound - (double)m) - l) : -INFINITY;
         }
     }
+    if (tid == 0) s_n = 0;
     __syncthreads();
-    /* every continuation left, to f(value, index): a wave a slice, and a thread a beam that ended */
-    auto each = [&](auto f) {
-        for (int i = wave; i < W * splits; i += PICK_THREADS / 64) {
-            const int b = i / splits;
-            const double score = s_score[b];
-            if (!(score > -INFINITY) || (a.ended && a.ended[group * W + b])) continue;
-            const int n = slices[i].count;
-            const float m = s_most[b];
-            for (int c = lane; c < n; c += 64) {
-                const beam_cand t = cands[(size_t)i * BEAM_CAP + c];
-                const double v = score + ((t.x == m ? 0.0 : (double)t.x - (double)m) - s_log[b]);
-                if (v > -INFINITY) f(v, (int64_t)b * V + t.v);
-            }
-        }
-        if (a.ended && tid < W && a.ended[group * W + tid] && s_score[tid] > -INFINITY) f(s_score[tid], (int64_t)tid * V + a.end_token);
+    double bound = s_bound[0];
+    for (int b = 1; b < W; b++) bound = fmax(bound, s_bound[b]);
+    /* every continuation that reaches the bound, to f(value, index) */
+    auto one = [&](int at, beam_cand t, auto f) {
+        const int b = at / row_cands;
+        const double score = s_score[b];
+        if (!(score > -INFINITY) || !(t.x > -INFINITY)) return;
+        const double v = score + ((t.x == s_most[b] ? 0.0 : (double)t.x - (double)s_most[b]) - s_log[b]);
+        if (v > -INFINITY && v >= bound) f(v, (int64_t)b * V + t.v);
     };
-    /* the range of the values, and how many there are */
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < PICK_HELD; r++)
+            if (tid + PICK_THREADS * r < total) one(tid + PICK_THREADS * r, held[r], f);
+        for (int at = tid + PICK_THREADS * PICK_HELD; at < total; at += PICK_THREADS) one(at, cands[at], f);
+        if (a.ended && tid < W && a.ended[group * W + tid]) {
+            const double v = (double)a.scores[group * W + tid];
+            if (v > -INFINITY && v >= bound) f(v, (int64_t)tid * V + a.end_token);
+        }
+    };
+    float* best = a.best + (size_t)group * K;
+    int *parents = a.parents + (size_t)group * K, *tokens = a.tokens + (size_t)group * K;
+    auto put = [&](int at, double v, int64_t i) {
+        best[at] = (float)v;
+        parents[at] = (int)(i / V);
+        tokens[at] = (int)(i % V);
+    };
+    auto none_from = [&](int n) {
+        for (int j = n + tid; j < K; j += PICK_THREADS) {
+            best[j] = -INFINITY;
+            parents[j] = -1;
+            tokens[j] = -1;
+        }
+    };
+    /* the n continuations of c_v and c_i to their places: several threads count those before one */
+    auto rank_all = [&](int n) {
+        int parts = 1;
+        while (parts < 16 && n * parts * 2 <= PICK_THREADS) parts *= 2;
+        for (int i = tid; i < n; i += PICK_THREADS) s_hist[i] = 0;
+        __syncthreads();
+        const int i = tid / parts;
+        if (i < n) {
+            const double v = c_v[i];
+            const int64_t at = c_i[i];
+            int before = 0;
+#pragma unroll 4
+            for (int j = tid % parts; j < n; j += parts) before += c_v[j] > v || (c_v[j] == v && c_i[j] < at);
+            if (before) atomicAdd(&s_hist[i], before);
+        }
+        __syncthreads();
+        if (tid < n && s_hist[tid] < K) put(s_hist[tid], c_v[tid], c_i[tid]);
+        none_from(n);
+    };
+    auto collect = [&](double v, int64_t i) {
+        const int at = atomicAdd(&s_n, 1); /* in any order: they are ranked */
+        if (at < PICK_CAP) { c_v[at] = v; c_i[at] = i; }
+    };
+    each(collect);
+    __syncthreads();
+    const int many = s_n, keep = min(K, many);
+    if (many <= PICK_CAP) {
+        rank_all(many);
+        return;
+    }
+
+    /* Many beams as good as each other, or many equal values: cut by their distance t to the largest, in bins; those with
+       t < from + width are kept, and the bin that holds the keep-th is cut again until they are few. */
     double most = -INFINITY, least = INFINITY;
-    int mine = 0;
     each([&](double v, int64_t) {
         most = fmax(most, v);
         least = fmin(least, v);
-        mine++;
     });
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         most = fmax(most, __shfl_xor(most, d, WAVE));
         least = fmin(least, __shfl_xor(least, d, WAVE));
-        mine += __shfl_xor(mine, d, WAVE);
     }
-    if (lane == 0) { r_v[wave] = most; r_i[wave] = __double_as_longlong(least); s_wave[wave] = mine; }
+    if (lane == 0) { r_v[wave] = most; r_i[wave] = __double_as_longlong(least); }
     __syncthreads();
-    int total = 0;
-    for (int w = 0; w < PICK_THREADS / 64; w++) {
+    for (int w = 0; w < PICK_WAVES; w++) {
         most = fmax(most, r_v[w]);
         least = fmin(least, __longlong_as_double(r_i[w]));
-        total += s_wave[w];
     }
-    const int keep = min(a.keep, total);
-    /* t(v) = how far v lies below the largest, 0 .. PICK_BINS of the range: those with t < from + width are kept, and
-       the bin that holds the keep-th is cut again until they are few */
     const double scale = most > least && most < INFINITY ? PICK_BINS / (most - least) : 0.0;
     auto below = [&](double v) { return v == most ? 0.0 : (most - v) * scale; };
     double from = 0.0, width = PICK_BINS + 1.0;
-    int before = 0, kept = total;
+    int before = 0, kept = many;
     for (int level = 0; level < 5 && kept > PICK_CAP; level++) {
         const double bins = PICK_BINS / width;
         for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_hist[i] = 0;
@@ -297,39 +363,20 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
         kept = s_n;
         __syncthreads();
     }
-    float* best = a.best + (size_t)group * a.keep;
-    int *parents = a.parents + (size_t)group * a.keep, *tokens = a.tokens + (size_t)group * a.keep;
-    auto put = [&](int at, double v, int64_t i) {
-        best[at] = (float)v;
-        parents[at] = (int)(i / V);
-        tokens[at] = (int)(i % V);
-    };
-    for (int i = keep + tid; i < a.keep; i += PICK_THREADS) {
-        best[i] = -INFINITY;
-        parents[i] = -1;
-        tokens[i] = -1;
-    }
     if (tid == 0) s_n = 0;
     __syncthreads();
     if (kept <= PICK_CAP) {
         each([&](double v, int64_t i) {
-            if (below(v) < from + width) {
-                const int at = atomicAdd(&s_n, 1);
-                if (at < PICK_CAP) { c_v[at] = v; c_i[at] = i; }
-            }
+            if (below(v) < from + width) collect(v, i);
         });
         __syncthreads();
-    }
-    const int n = s_n;
-    if (kept <= PICK_CAP && n <= PICK_CAP && n >= keep) {
-        if (tid < n) {
-            const double v = c_v[tid];
-            const int64_t i = c_i[tid];
-            int rank = 0;
-            for (int j = 0; j < n && rank < keep; j++) rank += c_v[j] > v || (c_v[j] == v && c_i[j] < i);
-            if (rank < keep) put(rank, v, i);
+        /* all above some value, so the keep best are among them if they are enough (a value on a bin's edge may fall to
+           either side) */
+        const int n = s_n;
+        if (n <= PICK_CAP && n >= keep) {
+            rank_all(n);
+            return;
         }
-        return;
     }
     /* more alike than can be ranked so: one a round */
     double last = INFINITY;
@@ -349,30 +396,34 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
         __syncthreads();
         if (lane == 0) { r_v[wave] = bv; r_i[wave] = bi; }
         __syncthreads();
-        for (int w = 0; w < PICK_THREADS / 64; w++)
+        for (int w = 0; w < PICK_WAVES; w++)
             if (r_v[w] > bv || (r_v[w] == bv && r_i[w] < bi)) { bv = r_v[w]; bi = r_i[w]; }
         if (tid == 0) put(round, bv, bi);
         last = bv;
         last_i = bi;
     }
+    none_from(keep);
 }
 
-/* Values a lane of the scan: 64 where that leaves two blocks a compute unit, else 16. */
-static int beam_lane_values(int rows, size_t vocab) { return (size_t)rows * vocab >= (size_t)512 * BEAM_WAVES * 64 * 64 ? 64 : 16; }
-static int beam_splits(int rows, size_t vocab) {
-    const size_t slice = (size_t)BEAM_WAVES * 64 * beam_lane_values(rows, vocab);
+/* Values a lane of the scan: 64 where that leaves most compute units a block, or where slices of 16 would leave more
+   candidates than the pick's threads hold; else 16. */
+static int beam_lane_values(int rows, int width, size_t vocab, int keep) {
+    const size_t small = (vocab + BEAM_WAVES * 64 * 16 - 1) / (BEAM_WAVES * 64 * 16);
+    return (size_t)rows * vocab >= (size_t)224 * BEAM_WAVES * 64 * 64 || width * small * keep > PICK_THREADS * PICK_HELD ? 64 : 16;
+}
+static int beam_splits(int rows, int width, size_t vocab, int keep) {
+    const size_t slice = (size_t)BEAM_WAVES * 64 * beam_lane_values(rows, width, vocab, keep);
     return (int)((vocab + slice - 1) / slice);
 }
 
 size_t beam_select_work(int groups, int width, size_t vocab, int keep) {
-    (void)keep;
-    const size_t rows = (size_t)groups * width, splits = beam_splits((int)rows, vocab);
-    return beam_slices_bytes(rows, splits) + rows * splits * BEAM_CAP * sizeof(beam_cand);
+    const size_t slices = (size_t)groups * width * beam_splits(groups * width, width, vocab, keep);
+    return beam_sums_bytes(slices) + slices * keep * sizeof(beam_cand);
 }
 
 hipError_t launch_beam_select(const beam_select_args& a, hipStream_t s) {
     if (a.groups < 1 || a.width < 1 || a.width > 64 || a.keep < 1 || a.keep > 64) return hipErrorInvalidValue;
-    const int rows = a.groups * a.width, splits = beam_splits(rows, a.vocab), E = beam_lane_values(rows, a.vocab);
+    const int rows = a.groups * a.width, splits = beam_splits(rows, a.width, a.vocab, a.keep), E = beam_lane_values(rows, a.width, a.vocab, a.keep);
     if ((size_t)rows * splits > ((size_t)1 << 23)) return hipErrorInvalidValue; /* threads of a launch stay within 32 bits */
     const int grid = rows * splits;
     const bool vec = ((uintptr_t)a.logits & 15) == 0 && a.stride % 4 == 0;
