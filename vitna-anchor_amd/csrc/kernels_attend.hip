@@ -253,15 +253,6 @@ __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(
 __device__ __forceinline__ int to_half_range(uint32_t mag) { return min(141 - (int)(mag >> 24), 126); }
 __device__ __forceinline__ float two_to(int k) { return __int_as_float((k + 127) << 23); } /* -126 .. 127 */
 
-/* Maximum over the wave, in every lane. */
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#define STEP_(C, RM) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, C, RM, 0xf, false))
-    STEP_(DPP_ROW_SHR(1), 0xf); STEP_(DPP_ROW_SHR(2), 0xf); STEP_(DPP_ROW_SHR(4), 0xf); STEP_(DPP_ROW_SHR(8), 0xf);
-    STEP_(DPP_ROW_BCAST15, 0xa); STEP_(DPP_ROW_BCAST31, 0xc);
-#undef STEP_
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
-}
-
 template <int HD, typename T, int NW>
 struct tile_shape {
     static constexpr bool PARTS = sizeof(T) == 4;                        /* operands in hi and lo */

@@ -20,7 +20,7 @@
    equal values) the block picks its keep one by one. */
 
 #define BEAM_WAVES 4
-#define BEAM_CAP 512
+#define BEAM_CAP 128 /* a wave's */
 
 /* float order as unsigned order, no NaN */
 __device__ __forceinline__ uint32_t beam_order(float x) {
@@ -28,10 +28,26 @@ __device__ __forceinline__ uint32_t beam_order(float x) {
     return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
+__device__ __forceinline__ unsigned long long beam_order64(double x) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(x);
+    return u ^ (u >> 63 ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double beam_value64(unsigned long long o) { return __longlong_as_double((long long)(o >> 63 ? o ^ (1ull << 63) : ~o)); }
+
+/* A continuation's place in the order of equal values: its beam, then its token (below 2^24). */
+__device__ __forceinline__ int beam_index(int b, int v) { return b << 24 | v; }
+
 struct beam_cand {
     float x; /* a logit, -inf: none */
     int v;   /* its token */
 };
+
+/* A candidate as one number: the earlier, the larger. */
+__device__ __forceinline__ uint64_t beam_key(float x, int v) { return (uint64_t)beam_order(x == 0.0f ? 0.0f : x) << 32 | (uint32_t)~v; }
+__device__ __forceinline__ beam_cand beam_of(uint64_t key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    return beam_cand{__uint_as_float(o >> 31 ? o ^ 0x80000000u : ~o), (int)~(uint32_t)key};
+}
 
 /* What beam_scan_kernel leaves: (maximum, sum) of [rows][splits], then beam_cand of [rows][splits][keep]. */
 static __host__ __device__ size_t beam_sums_bytes(size_t slices) { return (slices * sizeof(float2) + 255) & ~(size_t)255; }
@@ -43,8 +59,8 @@ template <int E, bool VEC>
 __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_args a, int splits) {
     __shared__ float sm[BEAM_WAVES], ss[BEAM_WAVES];
     __shared__ uint32_t st[BEAM_WAVES];
-    __shared__ int sn;
-    __shared__ beam_cand sc[BEAM_CAP];
+    __shared__ int sn[BEAM_WAVES];
+    __shared__ uint64_t sc[BEAM_WAVES][BEAM_CAP]; /* beam_key */
     const int split = blockIdx.x % splits, row = blockIdx.x / splits, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     if (a.ended && a.ended[row]) return; /* its one continuation needs no logits */
     beam_cand* out = reinterpret_cast<beam_cand*>(static_cast<char*>(a.work) + beam_sums_bytes((size_t)a.groups * a.width * splits)) +
@@ -54,17 +70,23 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
     /* value 4 e + j of a lane: VEC token first + 256 e + 4 lane + j, else first + 64 (4 e + j) + lane */
     auto token = [&](int e, int j) { return VEC ? first + 256 * e + 4 * lane + j : first + 64 * (4 * e + j) + lane; };
     float v[E / 4][4];
+    if (first + 64 * E <= V) {
 #pragma unroll
-    for (int e = 0; e < E / 4; e++) {
-        if (VEC && token(e, 3) < V) {
-            const float4 q = *reinterpret_cast<const float4*>(x + token(e, 0));
-            v[e][0] = q.x; v[e][1] = q.y; v[e][2] = q.z; v[e][3] = q.w;
-        } else {
+        for (int e = 0; e < E / 4; e++) {
+            if constexpr (VEC) {
+                const float4 q = *reinterpret_cast<const float4*>(x + token(e, 0));
+                v[e][0] = q.x; v[e][1] = q.y; v[e][2] = q.z; v[e][3] = q.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[e][j] = x[token(e, j)];
+            }
+        }
+    } else { /* the row's end */
+#pragma unroll
+        for (int e = 0; e < E / 4; e++)
 #pragma unroll
             for (int j = 0; j < 4; j++) v[e][j] = token(e, j) < V ? x[token(e, j)] : -INFINITY;
-        }
     }
-    if (tid == 0) sn = 0;
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int e = 0; e < E / 4; e++)
@@ -76,17 +98,24 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
     const float m = wave_max_dpp(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
     /* sum of exp(x - m): log2(e) in two parts, so that the argument is off by its own rounding alone */
     float s = 0.0f;
-    if (m > -INFINITY) {
+    if (m > -INFINITY && m < INFINITY) {
 #pragma unroll
         for (int e = 0; e < E / 4; e++) {
             float t[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float d = v[e][j] == m ? 0.0f : v[e][j] - m; /* (infinities) */
+                const float d = v[e][j] - m;
                 t[j] = __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f));
             }
             s += (t[0] + t[1]) + (t[2] + t[3]);
         }
+    } else if (m == INFINITY) { /* those alone count */
+#pragma unroll 1
+        for (int e = 0; e < E / 4; e++)
+            for (int j = 0; j < 4; j++) {
+                const int i = token(e, j);
+                if (i < V && x[i] == INFINITY) s += 1.0f;
+            }
     }
     s = wave_sum_dpp(s);
     /* the bound: the largest with at least keep of the wave's 256 maxima at or above it, nearly */
@@ -101,10 +130,7 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
     };
     {
         /* from the smallest of the lanes' maxima, which 64 of them reach */
-        uint32_t least = ~max(max(o[0], o[1]), max(o[2], o[3]));
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) least = max(least, (uint32_t)__shfl_xor((int)least, d, WAVE));
-        lo = ~least;
+        lo = ~wave_umax(~max(max(o[0], o[1]), max(o[2], o[3])));
         for (int step = 0; step < 20 && lo < hi; step++) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             const int n = above(mid);
@@ -122,7 +148,8 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
         st[wave] = lo;
     }
     __syncthreads();
-    lo = max(max(max(st[0], st[1]), max(st[2], st[3])), beam_order(-INFINITY) + 1);
+    lo = max(max(st[0], st[1]), max(st[2], st[3]));
+    const float bound = fmaxf(__uint_as_float(lo >> 31 ? lo ^ 0x80000000u : ~lo), -3.402823466e38f);
     if (tid == 0) {
         float M = -INFINITY, S = 0.0f;
         for (int w = 0; w < BEAM_WAVES; w++) M = fmaxf(M, sm[w]);
@@ -130,24 +157,71 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
             if (ss[w] > 0.0f) S += ss[w] * (sm[w] == M ? 1.0f : expf(sm[w] - M));
         static_cast<float2*>(a.work)[blockIdx.x] = make_float2(M, S);
     }
+    /* the wave's that reach it */
+    int mine = 0;
 #pragma unroll
     for (int e = 0; e < E / 4; e++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (beam_order(v[e][j]) >= lo) {
-                const int at = atomicAdd(&sn, 1); /* in any order: they are ranked */
-                if (at < BEAM_CAP) sc[at] = beam_cand{v[e][j], token(e, j)};
+        for (int j = 0; j < 4; j++) {
+            const uint64_t mask = __ballot(v[e][j] >= bound);
+            if (mask) {
+                const int at = mine + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+                if (v[e][j] >= bound && at < BEAM_CAP) sc[wave][at] = beam_key(v[e][j], token(e, j));
+                mine += __builtin_popcountll(mask);
             }
+        }
+    if (lane == 0) sn[wave] = mine;
     __syncthreads();
-    const int n = sn;
+    int n = 0, most = 0;
+#pragma unroll
+    for (int w = 0; w < BEAM_WAVES; w++) {
+        n += sn[w];
+        most = max(most, sn[w]);
+    }
     for (int i = n + tid; i < a.keep; i += 64 * BEAM_WAVES) out[i] = beam_cand{-INFINITY, INT32_MAX};
-    if (n <= BEAM_CAP) {
-        for (int i = tid; i < n; i += 64 * BEAM_WAVES) {
-            const beam_cand mine = sc[i];
-            int rank = 0;
-#pragma unroll 8
-            for (int j = 0; j < n; j++) rank += beam_before(sc[j].x, sc[j].v, mine.x, mine.v);
-            if (rank < a.keep) out[rank] = mine;
+    if (most <= BEAM_CAP) {
+        /* each wave its own in order, then a candidate's place among the others' by halving */
+        uint64_t key[BEAM_CAP / 64];
+        int rank[BEAM_CAP / 64];
+#pragma unroll
+        for (int u = 0; u < BEAM_CAP / 64; u++) {
+            key[u] = lane + 64 * u < mine ? sc[wave][lane + 64 * u] : 0;
+            rank[u] = 0;
+        }
+        int j = 0;
+        for (; j + 4 <= mine; j += 4) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint64_t other = sc[wave][j + q];
+#pragma unroll
+                for (int u = 0; u < BEAM_CAP / 64; u++) rank[u] += other > key[u] ? 1 : 0;
+            }
+        }
+        for (; j < mine; j++) {
+            const uint64_t other = sc[wave][j];
+#pragma unroll
+            for (int u = 0; u < BEAM_CAP / 64; u++) rank[u] += other > key[u] ? 1 : 0;
+        }
+        __builtin_amdgcn_wave_barrier(); /* LDS operations of one wave complete in order */
+#pragma unroll
+        for (int u = 0; u < BEAM_CAP / 64; u++)
+            if (lane + 64 * u < mine) sc[wave][rank[u]] = key[u];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < BEAM_CAP / 64; u++) {
+            if (lane + 64 * u >= mine || rank[u] >= a.keep) continue;
+            int place = rank[u];
+            for (int o = 1; o < BEAM_WAVES; o++) {
+                const int w = (wave + o) & (BEAM_WAVES - 1);
+                int lo_ = 0, hi_ = sn[w];
+                while (lo_ < hi_) {
+                    const int mid = (lo_ + hi_) >> 1;
+                    if (sc[w][mid] > key[u]) lo_ = mid + 1;
+                    else hi_ = mid;
+                }
+                place += lo_;
+            }
+            if (place < a.keep) out[place] = beam_of(key[u]);
         }
         return;
     }
@@ -187,29 +261,34 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
 
 #define PICK_THREADS 1024
 #define PICK_WAVES (PICK_THREADS / 64)
-#define PICK_HELD 8    /* candidates a thread asks for before anything else, and holds */
+#define PICK_HELD 7168 /* candidates that are kept in LDS */
 #define PICK_BINS 2048
-#define PICK_CAP 512   /* continuations that are ranked by counting */
+#define PICK_CAP 512   /* continuations that are ranked by counting, at most */
+#define PICK_FEW 96    /* and without cutting them first */
 
 __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_args a, int splits) {
+    __shared__ beam_cand s_cand[PICK_HELD];
     __shared__ double s_score[64], s_log[64]; /* of a beam: its score (-inf: it has no continuations), log of its sum of exponentials */
-    __shared__ double s_bound[64];            /* keep of its continuations are worth this or more */
+    __shared__ unsigned long long s_bound, s_top; /* keep of some beam's continuations are worth this or more; the best is worth (in order) */
     __shared__ float s_most[64];              /* its largest logit */
     __shared__ int s_hist[PICK_BINS], s_wave[PICK_WAVES], s_found[2], s_n;
     __shared__ double r_v[PICK_WAVES];
-    __shared__ int64_t r_i[PICK_WAVES];
+    __shared__ int r_i[PICK_WAVES];
     __shared__ double c_v[PICK_CAP];
-    __shared__ int64_t c_i[PICK_CAP];
+    __shared__ int c_i[PICK_CAP];
     const int group = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, W = a.width, K = a.keep;
     const size_t slices = (size_t)a.groups * W * splits;
     const float2* sums = static_cast<const float2*>(a.work) + (size_t)group * W * splits;
     const beam_cand* cands = reinterpret_cast<const beam_cand*>(static_cast<const char*>(a.work) + beam_sums_bytes(slices)) + (size_t)group * W * splits * K;
-    const int64_t V = (int64_t)a.vocab;
     const int row_cands = splits * K, total = W * row_cands;
-    beam_cand held[PICK_HELD];
-#pragma unroll
-    for (int r = 0; r < PICK_HELD; r++)
-        if (tid + PICK_THREADS * r < total) held[r] = cands[tid + PICK_THREADS * r];
+    if (tid == 0) {
+        s_bound = s_top = 0;
+        s_n = 0;
+    }
+    __syncthreads();
+    const bool held = total <= PICK_HELD;
+    if (held)
+        for (int i = tid; i < total; i += PICK_THREADS) s_cand[i] = cands[i];
     for (int b = wave; b < W; b += PICK_WAVES) {
         const int row = group * W + b;
         const float score = a.scores[row];
@@ -240,37 +319,35 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
             s_score[b] = on ? (double)score : -INFINITY;
             s_most[b] = m;
             s_log[b] = l;
-            s_bound[b] = on && bound > -INFINITY ? (double)score + ((bound == m ? 0.0 : (double)bound - (double)m) - l) : -INFINITY;
+            const double worth = (double)score + ((bound == m ? 0.0 : (double)bound - (double)m) - l);
+            if (on && bound > -INFINITY && worth == worth) atomicMax(&s_bound, beam_order64(worth));
+            const double best = ended ? (double)score : (double)score - l; /* of the largest logit */
+            if (score > -INFINITY && best == best) atomicMax(&s_top, beam_order64(best));
         }
     }
-    if (tid == 0) s_n = 0;
     __syncthreads();
-    double bound = s_bound[0];
-    for (int b = 1; b < W; b++) bound = fmax(bound, s_bound[b]);
+    const double bound = s_bound ? beam_value64(s_bound) : -INFINITY;
     /* every continuation that reaches the bound, to f(value, index) */
     auto one = [&](int at, beam_cand t, auto f) {
         const int b = at / row_cands;
         const double score = s_score[b];
         if (!(score > -INFINITY) || !(t.x > -INFINITY)) return;
         const double v = score + ((t.x == s_most[b] ? 0.0 : (double)t.x - (double)s_most[b]) - s_log[b]);
-        if (v > -INFINITY && v >= bound) f(v, (int64_t)b * V + t.v);
+        if (v > -INFINITY && v >= bound) f(v, beam_index(b, t.v));
     };
     auto each = [&](auto f) {
-#pragma unroll
-        for (int r = 0; r < PICK_HELD; r++)
-            if (tid + PICK_THREADS * r < total) one(tid + PICK_THREADS * r, held[r], f);
-        for (int at = tid + PICK_THREADS * PICK_HELD; at < total; at += PICK_THREADS) one(at, cands[at], f);
+        for (int at = tid; at < total; at += PICK_THREADS) one(at, held ? s_cand[at] : cands[at], f);
         if (a.ended && tid < W && a.ended[group * W + tid]) {
             const double v = (double)a.scores[group * W + tid];
-            if (v > -INFINITY && v >= bound) f(v, (int64_t)tid * V + a.end_token);
+            if (v > -INFINITY && v >= bound) f(v, beam_index(tid, a.end_token));
         }
     };
     float* best = a.best + (size_t)group * K;
     int *parents = a.parents + (size_t)group * K, *tokens = a.tokens + (size_t)group * K;
-    auto put = [&](int at, double v, int64_t i) {
+    auto put = [&](int at, double v, int i) {
         best[at] = (float)v;
-        parents[at] = (int)(i / V);
-        tokens[at] = (int)(i % V);
+        parents[at] = i >> 24;
+        tokens[at] = i & 0xffffff;
     };
     auto none_from = [&](int n) {
         for (int j = n + tid; j < K; j += PICK_THREADS) {
@@ -288,109 +365,98 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
         const int i = tid / parts;
         if (i < n) {
             const double v = c_v[i];
-            const int64_t at = c_i[i];
+            const int at = c_i[i];
             int before = 0;
-#pragma unroll 4
-            for (int j = tid % parts; j < n; j += parts) before += c_v[j] > v || (c_v[j] == v && c_i[j] < at);
+            int j = tid % parts;
+            for (; j + 3 * parts < n; j += 4 * parts) {
+                double w[4];
+                int k[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) { w[u] = c_v[j + u * parts]; k[u] = c_i[j + u * parts]; }
+#pragma unroll
+                for (int u = 0; u < 4; u++) before += (int)(w[u] > v) | ((int)(w[u] == v) & (int)(k[u] < at));
+            }
+            for (; j < n; j += parts) before += (int)(c_v[j] > v) | ((int)(c_v[j] == v) & (int)(c_i[j] < at));
             if (before) atomicAdd(&s_hist[i], before);
         }
         __syncthreads();
         if (tid < n && s_hist[tid] < K) put(s_hist[tid], c_v[tid], c_i[tid]);
         none_from(n);
     };
-    auto collect = [&](double v, int64_t i) {
-        const int at = atomicAdd(&s_n, 1); /* in any order: they are ranked */
-        if (at < PICK_CAP) { c_v[at] = v; c_i[at] = i; }
-    };
-    each(collect);
-    __syncthreads();
-    const int many = s_n, keep = min(K, many);
-    if (many <= PICK_CAP) {
-        rank_all(many);
-        return;
-    }
-
-    /* Many beams as good as each other, or many equal values: cut by their distance t to the largest, in bins; those with
-       t < from + width are kept, and the bin that holds the keep-th is cut again until they are few. */
-    double most = -INFINITY, least = INFINITY;
-    each([&](double v, int64_t) {
-        most = fmax(most, v);
-        least = fmin(least, v);
-    });
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        most = fmax(most, __shfl_xor(most, d, WAVE));
-        least = fmin(least, __shfl_xor(least, d, WAVE));
-    }
-    if (lane == 0) { r_v[wave] = most; r_i[wave] = __double_as_longlong(least); }
-    __syncthreads();
-    for (int w = 0; w < PICK_WAVES; w++) {
-        most = fmax(most, r_v[w]);
-        least = fmin(least, __longlong_as_double(r_i[w]));
-    }
+    /* Collected once whole; if they are many (beams as good as each other, equal values), they are cut by their distance t
+       to the largest, in bins: those with t < from + width are kept, the bin that holds the keep-th is cut again while
+       they are many, and the kept are collected. All of them lie above some value, so the keep best are among them if
+       they are enough (a value on a bin's edge may fall to either side). */
+    const double most = beam_value64(s_top), least = fmax(bound, most - 100.0);
     const double scale = most > least && most < INFINITY ? PICK_BINS / (most - least) : 0.0;
-    auto below = [&](double v) { return v == most ? 0.0 : (most - v) * scale; };
-    double from = 0.0, width = PICK_BINS + 1.0;
-    int before = 0, kept = many;
-    for (int level = 0; level < 5 && kept > PICK_CAP; level++) {
-        const double bins = PICK_BINS / width;
-        for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_hist[i] = 0;
-        if (tid == 0) { s_found[0] = 0; s_found[1] = before; s_n = kept; }
-        __syncthreads();
-        each([&](double v, int64_t) {
-            const double t = (below(v) - from) * bins;
-            if (t >= 0.0 && t < PICK_BINS) atomicAdd(&s_hist[(int)t], 1);
+    auto below = [&](double v) { return v == most ? 0.0 : fmin(fmax((most - v) * scale, 0.0), (double)PICK_BINS); };
+    double limit = INFINITY;
+    int keep = K;
+    for (bool whole = true;; whole = false) {
+        each([&](double v, int i) {
+            if (below(v) < limit) {
+                const int at = atomicAdd(&s_n, 1); /* in any order: they are ranked */
+                if (at < PICK_CAP) { c_v[at] = v; c_i[at] = i; }
+            }
         });
         __syncthreads();
-        /* two bins a thread: the bin where before + the counts so far reaches keep */
-        const int h0 = s_hist[2 * tid], h1 = s_hist[2 * tid + 1];
-        int run = h0 + h1;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(run, d, WAVE);
-            if (lane >= d) run += o;
-        }
-        if (lane == 63) s_wave[wave] = run;
-        __syncthreads();
-        int at = before;
-        for (int w = 0; w < wave; w++) at += s_wave[w];
-        const int b0 = at + run - h0 - h1, b1 = b0 + h0, b2 = b1 + h1; /* before bin 2 tid, before 2 tid + 1, behind it */
-        if (b0 < keep && b1 >= keep) { s_found[0] = 2 * tid; s_found[1] = b0; s_n = b1; }
-        if (b1 < keep && b2 >= keep) { s_found[0] = 2 * tid + 1; s_found[1] = b1; s_n = b2; }
-        __syncthreads();
-        from += s_found[0] / bins;
-        width /= PICK_BINS;
-        before = s_found[1];
-        kept = s_n;
-        __syncthreads();
-    }
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    if (kept <= PICK_CAP) {
-        each([&](double v, int64_t i) {
-            if (below(v) < from + width) collect(v, i);
-        });
-        __syncthreads();
-        /* all above some value, so the keep best are among them if they are enough (a value on a bin's edge may fall to
-           either side) */
-        const int n = s_n;
-        if (n <= PICK_CAP && n >= keep) {
-            rank_all(n);
+        const int many = s_n;
+        if (whole) keep = min(K, many);
+        if (many <= (whole ? PICK_FEW : PICK_CAP) && many >= keep) {
+            rank_all(many);
             return;
         }
+        if (!whole) break;
+        double from = 0.0, width = PICK_BINS + 1.0;
+        int before = 0, kept = many;
+        for (int level = 0; level < 5 && kept > PICK_FEW; level++) {
+            const double bins = PICK_BINS / width;
+            for (int i = tid; i < PICK_BINS; i += PICK_THREADS) s_hist[i] = 0;
+            if (tid == 0) { s_found[0] = 0; s_found[1] = before; s_n = kept; }
+            __syncthreads();
+            each([&](double v, int) {
+                const double t = (below(v) - from) * bins;
+                if (t >= 0.0 && t < PICK_BINS) atomicAdd(&s_hist[(int)t], 1);
+            });
+            __syncthreads();
+            /* two bins a thread: the bin where before + the counts so far reaches keep */
+            const int h0 = s_hist[2 * tid], h1 = s_hist[2 * tid + 1];
+            int run = h0 + h1;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(run, d, WAVE);
+                if (lane >= d) run += o;
+            }
+            if (lane == 63) s_wave[wave] = run;
+            __syncthreads();
+            int at = before;
+            for (int w = 0; w < wave; w++) at += s_wave[w];
+            const int b0 = at + run - h0 - h1, b1 = b0 + h0, b2 = b1 + h1; /* before bin 2 tid, before 2 tid + 1, behind it */
+            if (b0 < keep && b1 >= keep) { s_found[0] = 2 * tid; s_found[1] = b0; s_n = b1; }
+            if (b1 < keep && b2 >= keep) { s_found[0] = 2 * tid + 1; s_found[1] = b1; s_n = b2; }
+            __syncthreads();
+            from += s_found[0] / bins;
+            width /= PICK_BINS;
+            before = s_found[1];
+            kept = s_n;
+            __syncthreads();
+        }
+        limit = from + width;
+        if (tid == 0) s_n = 0;
+        __syncthreads();
     }
     /* more alike than can be ranked so: one a round */
     double last = INFINITY;
-    int64_t last_i = -1;
+    int last_i = -1;
     for (int round = 0; round < keep; round++) {
         double bv = -INFINITY;
-        int64_t bi = INT64_MAX;
-        each([&](double v, int64_t i) {
+        int bi = INT32_MAX;
+        each([&](double v, int i) {
             if ((v < last || (v == last && i > last_i)) && (v > bv || (v == bv && i < bi))) { bv = v; bi = i; }
         });
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const double v = __shfl_xor(bv, d, WAVE);
-            const int64_t i = __shfl_xor(bi, d, WAVE);
+            const int i = __shfl_xor(bi, d, WAVE);
             if (v > bv || (v == bv && i < bi)) { bv = v; bi = i; }
         }
         __syncthreads();
@@ -406,10 +472,10 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
 }
 
 /* Values a lane of the scan: 64 where that leaves most compute units a block, or where slices of 16 would leave more
-   candidates than the pick's threads hold; else 16. */
+   candidates than the pick holds in LDS; else 16. */
 static int beam_lane_values(int rows, int width, size_t vocab, int keep) {
     const size_t small = (vocab + BEAM_WAVES * 64 * 16 - 1) / (BEAM_WAVES * 64 * 16);
-    return (size_t)rows * vocab >= (size_t)224 * BEAM_WAVES * 64 * 64 || width * small * keep > PICK_THREADS * PICK_HELD ? 64 : 16;
+    return (size_t)rows * vocab >= (size_t)224 * BEAM_WAVES * 64 * 64 || width * small * keep > PICK_HELD ? 64 : 16;
 }
 static int beam_splits(int rows, int width, size_t vocab, int keep) {
     const size_t slice = (size_t)BEAM_WAVES * 64 * beam_lane_values(rows, width, vocab, keep);

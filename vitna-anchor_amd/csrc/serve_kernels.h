@@ -11,6 +11,15 @@
 
 #include "vitna_hip_internal.h"
 
+/* Maximum over the wave of unsigned numbers, in every lane. */
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#define STEP_(C, RM) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, C, RM, 0xf, false))
+    STEP_(DPP_ROW_SHR(1), 0xf); STEP_(DPP_ROW_SHR(2), 0xf); STEP_(DPP_ROW_SHR(4), 0xf); STEP_(DPP_ROW_SHR(8), 0xf);
+    STEP_(DPP_ROW_BCAST15, 0xa); STEP_(DPP_ROW_BCAST31, 0xc);
+#undef STEP_
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 #define ATTEND_G_MAX 16 /* query heads a key-value head */
 
 /* A row of the attention, as the caller's vitna_hip_attention_row_t. */
