@@ -6,6 +6,7 @@
 #include "serve_kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 /* ---- selection ----
    Two kernels. beam_scan_kernel reads each beam's logits once: a block takes a slice, and leaves the slice's maximum,
@@ -202,7 +203,9 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
 #pragma unroll
             for (int u = 0; u < BEAM_CAP / 64; u++) rank[u] += other > key[u] ? 1 : 0;
         }
-        __builtin_amdgcn_wave_barrier(); /* LDS operations of one wave complete in order */
+        /* LDS operations of one wave complete in order */
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int u = 0; u < BEAM_CAP / 64; u++)
             if (lane + 64 * u < mine) sc[wave][rank[u]] = key[u];
@@ -287,41 +290,62 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
     }
     __syncthreads();
     const bool held = total <= PICK_HELD;
-    if (held)
-        for (int i = tid; i < total; i += PICK_THREADS) s_cand[i] = cands[i];
-    for (int b = wave; b < W; b += PICK_WAVES) {
-        const int row = group * W + b;
-        const float score = a.scores[row];
-        const bool ended = a.ended && a.ended[row];
-        float2 t = make_float2(-INFINITY, 0.0f);
-        float bound = -INFINITY;
-        if (lane < splits) {
-            t = sums[b * splits + lane];
-            bound = cands[(b * splits + lane) * K + K - 1].x;
-        }
-        float m = t.x;
-        for (int i = lane + 64; i < splits; i += 64) {
-            m = fmaxf(m, sums[b * splits + i].x);
-            bound = fmaxf(bound, cands[(b * splits + i) * K + K - 1].x);
-        }
-        m = wave_max_dpp(m);
-        bound = wave_max_dpp(bound);
-        double s = t.y > 0.0f ? (double)(t.y * (t.x == m ? 1.0f : expf(t.x - m))) : 0.0;
-        for (int i = lane + 64; i < splits; i += 64) {
-            const float2 u = sums[b * splits + i];
-            if (u.y > 0.0f) s += (double)(u.y * (u.x == m ? 1.0f : expf(u.x - m)));
-        }
+    if (held) {
+        constexpr int N = PICK_HELD / PICK_THREADS;
+        beam_cand c[N]; /* all asked for at once */
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, WAVE);
-        if (lane == 0) {
-            const double l = log(s);
-            const bool on = score > -INFINITY && !ended; /* an ended beam's slices hold nothing */
+        for (int u = 0; u < N; u++)
+            if (tid + PICK_THREADS * u < total) c[u] = cands[tid + PICK_THREADS * u];
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            if (tid + PICK_THREADS * u < total) s_cand[tid + PICK_THREADS * u] = c[u];
+    }
+    /* sixteen lanes a beam */
+    {
+        const int b = tid >> 4, l = tid & 15, row = group * W + b;
+        const bool there = b < W;
+        const float score = there ? a.scores[row] : -INFINITY;
+        const bool ended = there && a.ended && a.ended[row]; /* its slices hold nothing */
+        float2 t[4];
+        float least = -INFINITY, m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            t[u] = make_float2(-INFINITY, 0.0f);
+            if (there && l + 16 * u < splits) {
+                t[u] = sums[b * splits + l + 16 * u];
+                least = fmaxf(least, cands[(b * splits + l + 16 * u) * K + K - 1].x);
+            }
+            m = fmaxf(m, t[u].x);
+        }
+        if (there)
+            for (int i = l + 64; i < splits; i += 16) {
+                m = fmaxf(m, sums[b * splits + i].x);
+                least = fmaxf(least, cands[(b * splits + i) * K + K - 1].x);
+            }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            m = fmaxf(m, __shfl_xor(m, d, WAVE));
+            least = fmaxf(least, __shfl_xor(least, d, WAVE));
+        }
+        double s = 0.0;
+        auto add = [&](float2 u) {
+            if (u.y > 0.0f) s += (double)(u.y * (u.x == m ? 1.0f : expf(u.x - m)));
+        };
+#pragma unroll
+        for (int u = 0; u < 4; u++) add(t[u]);
+        if (there)
+            for (int i = l + 64; i < splits; i += 16) add(sums[b * splits + i]);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) s += __shfl_xor(s, d, WAVE);
+        if (there && l == 0) {
+            const double log_s = log(s);
+            const bool on = score > -INFINITY && !ended;
             s_score[b] = on ? (double)score : -INFINITY;
             s_most[b] = m;
-            s_log[b] = l;
-            const double worth = (double)score + ((bound == m ? 0.0 : (double)bound - (double)m) - l);
-            if (on && bound > -INFINITY && worth == worth) atomicMax(&s_bound, beam_order64(worth));
-            const double best = ended ? (double)score : (double)score - l; /* of the largest logit */
+            s_log[b] = log_s;
+            const double worth = (double)score + ((least == m ? 0.0 : (double)least - (double)m) - log_s);
+            if (on && least > -INFINITY && worth == worth) atomicMax(&s_bound, beam_order64(worth));
+            const double best = ended ? (double)score : (double)score - log_s; /* of the largest logit */
             if (score > -INFINITY && best == best) atomicMax(&s_top, beam_order64(best));
         }
     }
@@ -504,49 +528,71 @@ hipError_t launch_beam_select(const beam_select_args& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-/* ---- reordering ---- */
+/* ---- reordering ----
+   A thread takes the same few bytes of every beam of a group: all that moves is read before any is written, so a beam
+   may take another's place while that takes a third's, and no thread waits for another. What it takes lies at the same
+   place in every layer, so a block walks over layers with its beams and offsets at hand. Bound by memory: half a beam's
+   worth is read and half written for each that changes. */
 
-/* A thread takes the same 16 bytes of every beam of a group: all it needs are read before any is written, so a beam
-   may take another's place while that takes a third's, and no thread waits for another. */
+/* the bytes a thread takes of a beam: what W of them leave room for in registers */
+template <int W>
+using reorder_piece = std::conditional_t<W <= 32, u32x4, uint2>;
+
 template <int W>
 __global__ __launch_bounds__(256) void kv_reorder_kernel(kv_reorder_args a) {
-    const int group = blockIdx.z, layer = blockIdx.y >> 1;
-    char* cache = (blockIdx.y & 1 ? a.v : a.k) + (size_t)layer * a.layer_bytes;
-    const int from = max(a.spans[2 * group], 0), to = min(a.spans[2 * group + 1], a.ctx);
-    const int head_pieces = (int)(a.dim_bytes / 16), pieces = a.n_kv * head_pieces;
-    const int64_t many = to > from ? (int64_t)(to - from) * pieces : 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < many; i += (int64_t)gridDim.x * 256) {
-        const int64_t pos = from + i / pieces;
-        const int piece = (int)(i % pieces);
-        const size_t at = (size_t)pos * a.pos_bytes + (size_t)(piece / head_pieces) * a.head_bytes + (size_t)(piece % head_pieces) * 16;
-        u32x4 v[W];
-        bool on[W];
-#pragma unroll
-        for (int b = 0; b < W; b++) {
-            on[b] = false;
-            if (b < a.width) {
-                const int p = a.parents[group * a.width + b], to_seq = a.list[group * a.width + b];
-                if (p >= 0 && p < a.width && p != b && to_seq >= 0 && to_seq < a.seqs) {
-                    const int seq = a.list[group * a.width + p];
-                    if (seq >= 0 && seq < a.seqs) {
-                        on[b] = true;
-                        v[b] = *reinterpret_cast<const u32x4*>(cache + (size_t)seq * a.seq_bytes + at);
-                    }
-                }
-            }
+    typedef reorder_piece<W> piece_t;
+    __shared__ int s_from[W], s_to[W];
+    const int group = blockIdx.z, tid = threadIdx.x;
+    if (tid < W) {
+        int from = -1, to = -1;
+        if (tid < a.width) {
+            const int p = a.parents[group * a.width + tid];
+            to = a.list[group * a.width + tid];
+            if (p >= 0 && p < a.width && p != tid) from = a.list[group * a.width + p];
+            if (from < 0 || from >= a.seqs || to < 0 || to >= a.seqs) from = -1;
         }
-#pragma unroll
-        for (int b = 0; b < W; b++)
-            if (on[b]) *reinterpret_cast<u32x4*>(cache + (size_t)a.list[group * a.width + b] * a.seq_bytes + at) = v[b];
+        s_from[tid] = from;
+        s_to[tid] = to;
     }
+    const int first = max(a.spans[2 * group], 0), last = min(a.spans[2 * group + 1], a.ctx);
+    const int head_pieces = (int)(a.dim_bytes / sizeof(piece_t)), pieces = a.n_kv * head_pieces;
+    const int64_t many = last > first ? (int64_t)(last - first) * pieces : 0;
+    __syncthreads();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < many; i += (int64_t)gridDim.x * 256) {
+        const int64_t pos = many <= INT32_MAX ? first + (int)i / pieces : first + i / pieces;
+        const int piece = (int)(i - (pos - first) * pieces);
+        const size_t at = (size_t)pos * a.pos_bytes + (size_t)(piece / head_pieces) * a.head_bytes + (size_t)(piece % head_pieces) * sizeof(piece_t);
+        for (int y = blockIdx.y; y < 2 * a.layers; y += gridDim.y) {
+            char* cache = (y & 1 ? a.v : a.k) + (size_t)(y >> 1) * a.layer_bytes + at;
+            piece_t v[W];
+#pragma unroll
+            for (int b = 0; b < W; b++) {
+                const int from = __builtin_amdgcn_readfirstlane(s_from[b]);
+                if (from >= 0) v[b] = *reinterpret_cast<const piece_t*>(cache + (size_t)from * a.seq_bytes);
+            }
+#pragma unroll
+            for (int b = 0; b < W; b++)
+                if (__builtin_amdgcn_readfirstlane(s_from[b]) >= 0)
+                    *reinterpret_cast<piece_t*>(cache + (size_t)__builtin_amdgcn_readfirstlane(s_to[b]) * a.seq_bytes) = v[b];
+        }
+    }
+}
+
+template <int W>
+static void reorder(const kv_reorder_args& a, hipStream_t s) {
+    /* blocks over the positions, then over the layers until there are eight a compute unit */
+    const int64_t pieces = (int64_t)a.longest * a.n_kv * (int64_t)(a.dim_bytes / sizeof(reorder_piece<W>));
+    const unsigned x = (unsigned)std::min<int64_t>(std::max<int64_t>((pieces + 255) / 256, 1), 4096);
+    const int64_t want = 2048 / ((int64_t)x * a.groups) + 1;
+    kv_reorder_kernel<W><<<dim3(x, (unsigned)std::min<int64_t>(2 * a.layers, want), a.groups), 256, 0, s>>>(a);
 }
 
 hipError_t launch_kv_reorder(const kv_reorder_args& a, hipStream_t s) {
     if (a.groups < 1 || a.width < 1 || a.width > 64 || a.layers < 1 || a.dim_bytes % 16) return hipErrorInvalidValue;
-    const int64_t pieces = (int64_t)a.longest * a.n_kv * (int64_t)(a.dim_bytes / 16);
-    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>((pieces + 255) / 256, 1), 4096), 2 * a.layers, a.groups);
-    if (a.width <= 4) kv_reorder_kernel<4><<<grid, 256, 0, s>>>(a);
-    else if (a.width <= 16) kv_reorder_kernel<16><<<grid, 256, 0, s>>>(a);
-    else kv_reorder_kernel<64><<<grid, 256, 0, s>>>(a);
+    if (a.width <= 4) reorder<4>(a, s);
+    else if (a.width <= 8) reorder<8>(a, s);
+    else if (a.width <= 16) reorder<16>(a, s);
+    else if (a.width <= 32) reorder<32>(a, s);
+    else reorder<64>(a, s);
     return hipGetLastError();
 }
