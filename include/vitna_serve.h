@@ -32,7 +32,8 @@ extern "C" {
 /** A layer's key-value cache of several sequences, and how it is read.
     Element (sequence, position, head, d) of the keys and of the values lies
     seq * seq_stride + pos * pos_stride + head * head_stride + d elements
-    behind k and v. k, v and every stride are whole multiples of 16 bytes. */
+    behind k and v. k, v and every stride are whole multiples of 16 bytes,
+    pos_stride at most 2^23 elements. */
 typedef struct {
     const void* k;             /* DEVICE */
     const void* v;             /* DEVICE */

@@ -39,7 +39,7 @@ VIEWS = [
     (dict(dtype=va.Q8_0), "dtype"), (dict(head_dim=96), "dimensions"), (dict(n_heads=7), "query heads"), (dict(n_heads=34), "query heads"),
     (dict(n_kv_heads=0, n_heads=0, pos_stride=256), "key-value heads"), (dict(n_heads=0), "query heads"), (dict(ctx=0), "positions"),
     (dict(ctx=(1 << 30) + 1), "positions"), (dict(seqs=0), "sequences"), (dict(seqs=1 << 31), "sequences"),
-    (dict(pos_stride=258), "strides"), (dict(dtype=va.BF16, head_stride=132), "strides"), (dict(seq_stride=1 << 60), "too large"),
+    (dict(pos_stride=258), "strides"), (dict(dtype=va.BF16, head_stride=132), "strides"), (dict(seq_stride=1 << 60), "too large"), (dict(pos_stride=(1 << 23) + 4), "positions 8388612 elements apart"),
     (dict(k=AT + 4), "aligned"), (dict(v=AT + 8), "aligned"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(scale=float("inf")), "scale"),
 ]

@@ -246,6 +246,12 @@ __device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, flo
     lo = make_uint2(pack_cut(fmaf(x0, s, -half_lo(hi.x)), fmaf(x1, s, -half_hi(hi.x))), pack_cut(fmaf(x2, s, -half_lo(hi.y)), fmaf(x3, s, -half_hi(hi.y))));
 }
 
+__device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, uint2& hi, uint2& lo) {
+    hi = make_uint2(pack_cut(x0, x1), pack_cut(x2, x3));
+    lo = make_uint2(pack_cut(fmaf(half_lo(hi.x), -1.0f, x0), fmaf(half_hi(hi.x), -1.0f, x1)),
+                    pack_cut(fmaf(half_lo(hi.y), -1.0f, x2), fmaf(half_hi(hi.y), -1.0f, x3)));
+}
+
 /* Values as keys for a maximum of magnitudes: the sign shifted out, so a NaN is the largest, then an infinity. */
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) << 1; }
 #define MAG_INF 0xff000000u
@@ -272,9 +278,18 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
     constexpr int KS = HD / 16, DT = HD / 32, U = sh::U, CC = sh::CC, HALF = sh::HALF;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c32 = lane & 31, hh = lane >> 5;
     const int G = a.n_heads / a.n_kv, TR = 32 * NW / G, r0 = tile * TR, nr = min(TR, a.n - r0);
-    _Float16* sk = reinterpret_cast<_Float16*>(lds);       /* [part][64 positions][HD], pieces of 8 swizzled by position */
-    _Float16* sv = sk + (PARTS ? 2 : 1) * HALF;            /* [part][HD][64 positions], pieces of 4 + 4 swizzled by dimension */
-    attend_row* srow = reinterpret_cast<attend_row*>(sv + (PARTS ? 2 : 1) * HALF);
+    /* Keys [part][64 positions][HD] in pieces of 8 dimensions, piece x of position t at x ^ t mod (HD / 8). Values
+       [part][HD][64 positions] in units of two pieces of 4 positions, those of one MFMA operand (positions 16 s + 4 hh ..
+       and 16 s + 8 + 4 hh ..: unit 2 s + hh), unit x of dimension d at x ^ (d / 2 ^ d / 16) mod 8. Sixteen lanes'
+       16-byte reads then take every bank once, and all places are one lane's ^ and + a constant. */
+    char* sk = lds;
+    char* sv = sk + (PARTS ? 2 : 1) * HALF * 2;
+    attend_row* srow = reinterpret_cast<attend_row*>(sv + (PARTS ? 2 : 1) * HALF * 2);
+    auto key_to = [&](int pg, int cc) { return (uint32_t)(4 * pg * HD * 2 + (((cc >> 1) ^ ((4 * pg) & (HD / 8 - 1))) << 4) + 8 * (cc & 1)); };
+    auto value_to = [&](int pg, int cc) {
+        const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1;
+        return (uint32_t)(4 * cc * 128 + ((unit ^ (((2 * cc) ^ (cc >> 2)) & 7)) << 4) + 8 * half);
+    };
     uint32_t* smax = reinterpret_cast<uint32_t*>(srow + sh::ROWS); /* [2][NW]: magnitudes of keys, of values */
     uint32_t* sbad = smax + 2 * NW;                        /* positions whose values are not finite */
 
@@ -294,7 +309,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
         const float* at = a.q + (size_t)(r0 + (there ? lr : 0)) * a.q_stride + (size_t)(h * G + g) * HD + 8 * hh;
         /* read twice: kept between, the values would take the registers that the loop needs */
         uint32_t mag = 0;
-#pragma unroll 2
+#pragma unroll
         for (int s = 0; s < 2 * KS; s++) {
             const float4 x = *reinterpret_cast<const float4*>(at + 16 * (s >> 1) + 4 * (s & 1));
             mag = max(max(mag, max(magnitude(x.x), magnitude(x.y))), max(magnitude(x.z), magnitude(x.w)));
@@ -313,6 +328,10 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
             ql[s] = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
         }
     }
+    const char* key_at = sk + c32 * HD * 2;
+    const uint32_t key_x = (hh ^ (c32 & (HD / 8 - 1))) << 4; /* piece 2 s + hh: ^ s << 5 */
+    const char* value_at = sv + c32 * 128;
+    const uint32_t value_x = (hh ^ ((c32 >> 1) & 7) ^ (c32 >> 4)) << 4; /* unit 2 s + hh of dimension 32 d + c32: ^ (s ^ d) << 5 */
     float m_run = -INFINITY, l_run = 0.0f;
     int e_run = 126, e_out = 126; /* the values' power of two, of the block and in this wave's O */
     f16v O[DT];
@@ -323,6 +342,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
 
     const T* kh = (const T*)a.k + (size_t)h * a.head_stride;
     const T* vh = (const T*)a.v + (size_t)h * a.head_stride;
+    const uint32_t pos_bytes = (uint32_t)(a.pos_stride * sizeof(T)); /* 64 of them stay within 31 bits */
     int first = 0;
     while (first < nr) {
         /* rows first .. next - 1 read the same positions of the same sequence */
@@ -371,17 +391,17 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
         auto start = [&](int c) { return c < n_sink ? 64 * c : from + 64 * (c - n_sink); };
         auto stop = [&](int c) { return c < n_sink ? sink : end; };
         vec<T, 4> rk[U][4], rv[U][4];
+        /* (positions behind the chunk's end read its last again: their scores are masked) */
         auto fetch = [&](const T* src, int c, vec<T, 4> (&x)[U][4]) {
-            const int t0 = start(c), t1 = stop(c);
+            const int t0 = start(c);
+            const uint32_t most = (uint32_t)(min(stop(c) - t0, 64) - 1);
+            const char* from_ = reinterpret_cast<const char*>(src + (size_t)t0 * a.pos_stride);
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int at = tid + sh::NT * u, pg = at / CC, cc = at % CC;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int t = t0 + 4 * pg + i;
-                    if (t < t1) x[u][i] = *reinterpret_cast<const vec<T, 4>*>(src + (size_t)t * a.pos_stride + 4 * cc);
-                    else x[u][i] = vec<T, 4>{};
-                }
+                for (int i = 0; i < 4; i++)
+                    x[u][i] = *reinterpret_cast<const vec<T, 4>*>(from_ + (min((uint32_t)(4 * pg + i), most) * pos_bytes + (uint32_t)(4 * sizeof(T)) * cc));
             }
         };
         auto publish = [&](const vec<T, 4> (&x)[U][4], uint32_t* to) {
@@ -431,7 +451,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                 float f = 1.0f;
                 if constexpr (SCALED) {
                     uint32_t mag = largest(smax);
-                    if (mag >= MAG_INF) mag = finite_largest(rk, smax);
+                    if (__builtin_expect(mag >= MAG_INF, 0)) mag = finite_largest(rk, smax);
                     const int k = to_half_range(mag);
                     f = two_to(k);
                     from_keys = fmaxf(to_score * two_to(-k), 1e-37f); /* (a masked score's -inf times 0 would be NaN) */
@@ -441,7 +461,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                     const int at = tid + sh::NT * u, pg = at / CC, cc = at % CC;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int pos = 4 * pg + i, to = pos * HD + (((cc >> 1) ^ (pos & (HD / 8 - 1))) * 8) + 4 * (cc & 1);
+                        const uint32_t to = (key_to(pg, cc) ^ (i << 4)) + i * HD * 2;
                         uint2 hi, lo;
                         if constexpr (SCALED) {
                             cut4((float)rk[u][i][0], (float)rk[u][i][1], (float)rk[u][i][2], (float)rk[u][i][3], f, hi, lo);
@@ -449,7 +469,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                             hi = __builtin_bit_cast(uint2, rk[u][i]);
                         }
                         *reinterpret_cast<uint2*>(sk + to) = hi;
-                        if constexpr (PARTS) *reinterpret_cast<uint2*>(sk + HALF + to) = lo;
+                        if constexpr (PARTS) *reinterpret_cast<uint2*>(sk + HALF * 2 + to) = lo;
                     }
                 }
             }
@@ -463,15 +483,14 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                     f16v acc;
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[i] = 0.0f;
-                    const int pos = 32 * pt + c32;
 #pragma unroll
                     for (int s = 0; s < KS; s++) {
-                        const int at = pos * HD + ((2 * s + hh) ^ (pos & (HD / 8 - 1))) * 8;
-                        const h8v k8 = *reinterpret_cast<const h8v*>(sk + at);
+                        const char* at = key_at + (key_x ^ (s << 5)) + 32 * pt * HD * 2;
+                        const h8v k8 = *reinterpret_cast<const h8v*>(at);
                         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[s], acc, 0, 0, 0);
                         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[s], acc, 0, 0, 0);
                         if constexpr (PARTS) {
-                            const h8v kl = *reinterpret_cast<const h8v*>(sk + HALF + at);
+                            const h8v kl = *reinterpret_cast<const h8v*>(at + HALF * 2);
                             acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[s], acc, 0, 0, 0);
                         }
                     }
@@ -482,7 +501,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
             float to_half = 1.0f;
             uint32_t mag = largest(smax + NW);
             const bool bad = mag >= MAG_INF;
-            if (bad) {
+            if (__builtin_expect(bad, 0)) {
                 mag = finite_largest(rv, smax + NW);
 #pragma unroll
                 for (int u = 0; u < U; u++) {
@@ -509,12 +528,14 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                 /* lane: positions t0 + 32 pt + 8 (i / 4) + 4 hh + i % 4 of its column */
                 const bool whole = !__any(on && !(t0 + 64 <= t1 && t0 + 63 <= last && (t0 >= low || t0 + 64 <= a.sinks))) && __all(on);
                 if (!whole) {
+                    /* of the lane's positions, t0 + 4 hh + 32 pt + 8 (i / 4) + i % 4 */
+                    const int to_last = on ? min(last, t1 - 1) - t0 - 4 * hh : -1, to_low = max(low, -1) - t0 - 4 * hh, to_sink = a.sinks - t0 - 4 * hh;
 #pragma unroll
                     for (int pt = 0; pt < 2; pt++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const int t = t0 + 32 * pt + 8 * (i >> 2) + 4 * hh + (i & 3);
-                            const bool sees = on && t < t1 && t <= last && (t >= low || t < a.sinks);
+                            const int t = 32 * pt + 8 * (i >> 2) + (i & 3);
+                            const bool sees = t <= to_last && (t >= to_low || t < to_sink);
                             S[pt][i] = sees ? S[pt][i] : -INFINITY;
                         }
                 }
@@ -529,16 +550,20 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                 float f = exp2_hw(m_run - base);
                 const float up = 14.0f - base; /* weights up to 2^14 */
                 float l = 0.0f;
-                uint32_t poison[2] = {0, 0};
-                if (bad) {
-                    poison[0] = sbad[0];
-                    poison[1] = sbad[1];
+                if (__builtin_expect(bad, 0)) {
+                    for (int pt = 0; pt < 2; pt++) {
+                        const uint32_t poison = sbad[pt];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float x = pt ? S[1][i] : S[0][i];
+                            if (((poison >> (8 * (i >> 2) + 4 * hh + (i & 3))) & 1) && !(x == -INFINITY)) l = NAN;
+                        }
+                    }
                 }
 #pragma unroll
                 for (int pt = 0; pt < 2; pt++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        if (bad && ((poison[pt] >> (8 * (i >> 2) + 4 * hh + (i & 3))) & 1) && !(S[pt][i] == -INFINITY)) l = NAN;
                         S[pt][i] = exp2_hw(fmaf(S[pt][i], from_keys, up));
                         l += S[pt][i];
                     }
@@ -559,10 +584,9 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int at = tid + sh::NT * u, pg = at / CC, cc = at % CC;
-                const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1;
 #pragma unroll
                 for (int d = 0; d < 4; d++) {
-                    const int dim = 4 * cc + d, to = dim * 64 + ((unit ^ (((dim >> 1) ^ (dim >> 4)) & 7)) * 8) + 4 * half;
+                    const uint32_t to = (value_to(pg, cc) ^ ((d >> 1) << 4)) + d * 128;
                     uint2 hi, lo;
                     if constexpr (SCALED) {
                         cut4((float)rv[u][0][d], (float)rv[u][1][d], (float)rv[u][2][d], (float)rv[u][3][d], to_half, hi, lo);
@@ -570,7 +594,7 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                         hi = __builtin_bit_cast(uint2, vec<T, 4>{rv[u][0][d], rv[u][1][d], rv[u][2][d], rv[u][3][d]});
                     }
                     *reinterpret_cast<uint2*>(sv + to) = hi;
-                    if constexpr (PARTS) *reinterpret_cast<uint2*>(sv + HALF + to) = lo;
+                    if constexpr (PARTS) *reinterpret_cast<uint2*>(sv + HALF * 2 + to) = lo;
                 }
             }
             if constexpr (SCALED) {
@@ -586,17 +610,17 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                     const f16v& P = S[s >> 1];
                     const int o = 8 * (s & 1);
                     uint2 h0, l0, h1, l1;
-                    cut4(P[o], P[o + 1], P[o + 2], P[o + 3], 1.0f, h0, l0);
-                    cut4(P[o + 4], P[o + 5], P[o + 6], P[o + 7], 1.0f, h1, l1);
+                    cut4(P[o], P[o + 1], P[o + 2], P[o + 3], h0, l0);
+                    cut4(P[o + 4], P[o + 5], P[o + 6], P[o + 7], h1, l1);
                     const h8v ph = __builtin_bit_cast(h8v, u32x4{h0.x, h0.y, h1.x, h1.y}), pl = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
 #pragma unroll
                     for (int d = 0; d < DT; d++) {
-                        const int dim = 32 * d + c32, at = dim * 64 + ((2 * s + hh) ^ (((dim >> 1) ^ (dim >> 4)) & 7)) * 8;
-                        const h8v v8 = *reinterpret_cast<const h8v*>(sv + at);
+                        const char* at = value_at + (value_x ^ ((s ^ d) << 5)) + 32 * d * 128;
+                        const h8v v8 = *reinterpret_cast<const h8v*>(at);
                         O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, O[d], 0, 0, 0);
                         O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, O[d], 0, 0, 0);
                         if constexpr (PARTS) {
-                            const h8v vl = *reinterpret_cast<const h8v*>(sv + HALF + at);
+                            const h8v vl = *reinterpret_cast<const h8v*>(at + HALF * 2);
                             O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, O[d], 0, 0, 0);
                         }
                     }
@@ -667,47 +691,86 @@ __global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_shared_kernel(a
     }
 }
 
-/* A block a (row, key-value head): the parts' factors in LDS, then four dimensions of a head a thread. */
+/* HB heads of a row a block, SG threads for each four dimensions of one: the parts' factors once in LDS, then each
+   thread adds up every SG-th part, all its loads asked for before the first is used. */
 #define MERGE_SPLITS 512 /* parts of a row at most */
-template <int HD>
+#define MERGE_AHEAD 8
+template <int HD, int SG>
 __global__ __launch_bounds__(256) void attend_merge_kernel(attend_args a, attend_parts p) {
-    __shared__ float sf[MERGE_SPLITS * ATTEND_G_MAX];
-    const int G = a.n_heads / a.n_kv, S = p.own + p.tile, tid = threadIdx.x, h = blockIdx.x % a.n_kv, row = blockIdx.x / a.n_kv;
-    const size_t part = ((size_t)row * a.n_kv + h) * S;
-    /* a wave a few heads: the maximum, the sum, and each part's factor */
-    for (int g = tid >> 6; g < G; g += 4) {
-        const int lane = tid & 63;
-        float m = -INFINITY;
-        for (int s = lane; s < S; s += 64) {
-            const float2 x = p.ml[(part + s) * G + g];
-            if (x.y != 0.0f) m = fmaxf(m, x.x);
-        }
-        m = wave_max_dpp(m);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        for (int s = lane; s < S; s += 64) {
-            const float2 x = p.ml[(part + s) * G + g];
-            if (x.y != 0.0f) l = fmaf(x.y, exp2_hw(x.x - base), l);
-        }
-        l = wave_sum_dpp(l);
-        for (int s = lane; s < S; s += 64) {
-            const float2 x = p.ml[(part + s) * G + g];
-            sf[s * G + g] = x.y != 0.0f ? exp2_hw(x.x - base) / l : 0.0f;
+    constexpr int D = HD / 4, HB = 256 / D / SG;
+    __shared__ float sf[HB][MERGE_SPLITS];
+    __shared__ float4 so[SG > 1 ? 256 : 1];
+    const int G = a.n_heads / a.n_kv, S = p.own + p.tile, tid = threadIdx.x, blocks = (a.n_heads + HB - 1) / HB;
+    const int row = blockIdx.x / blocks, head0 = blockIdx.x % blocks * HB;
+    /* a head's parts: of key-value head head / G, split s, at ((row n_kv + head / G) S + s) G + head % G */
+    auto part = [&](int head, int s) { return (((size_t)row * a.n_kv + head / G) * S + s) * G + head % G; };
+    constexpr int LF = 256 / HB < 64 ? 256 / HB : 64; /* lanes for a head's factors */
+    {
+        const int at = tid / LF, l = tid % LF, head = head0 + at;
+        if (at < HB && head < a.n_heads) {
+            float2 x[2];
+            float m = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                x[u] = l + LF * u < S ? p.ml[part(head, l + LF * u)] : make_float2(-INFINITY, 0.0f);
+                if (x[u].y != 0.0f) m = fmaxf(m, x[u].x);
+            }
+            for (int s = l + 2 * LF; s < S; s += LF) {
+                const float2 y = p.ml[part(head, s)];
+                if (y.y != 0.0f) m = fmaxf(m, y.x);
+            }
+#pragma unroll
+            for (int d = 1; d < LF; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, WAVE));
+            const float base = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (x[u].y != 0.0f) sum = fmaf(x[u].y, exp2_hw(x[u].x - base), sum);
+            for (int s = l + 2 * LF; s < S; s += LF) {
+                const float2 y = p.ml[part(head, s)];
+                if (y.y != 0.0f) sum = fmaf(y.y, exp2_hw(y.x - base), sum);
+            }
+#pragma unroll
+            for (int d = 1; d < LF; d <<= 1) sum += __shfl_xor(sum, d, WAVE);
+            const float inv = 1.0f / sum;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (l + LF * u < S) sf[at][l + LF * u] = x[u].y != 0.0f ? exp2_hw(x[u].x - base) * inv : 0.0f;
+            for (int s = l + 2 * LF; s < S; s += LF) {
+                const float2 y = p.ml[part(head, s)];
+                sf[at][s] = y.y != 0.0f ? exp2_hw(y.x - base) * inv : 0.0f;
+            }
         }
     }
     __syncthreads();
-    for (int i = tid; i < G * HD / 4; i += 256) {
-        const int g = i / (HD / 4), d = i % (HD / 4);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < S; s++) {
-            const float f = sf[s * G + g];
-            if (f != 0.0f) { /* a part without a sum has no values */
-                const float4 x = reinterpret_cast<const float4*>(p.acc + ((part + s) * G + g) * HD)[d];
-                o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+    const int d = tid % D, sg = tid / D % SG, at = tid / D / SG, head = head0 + at;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (head < a.n_heads) {
+        for (int s0 = sg; s0 < S; s0 += SG * MERGE_AHEAD) {
+            float4 x[MERGE_AHEAD];
+#pragma unroll
+            for (int u = 0; u < MERGE_AHEAD; u++)
+                if (s0 + SG * u < S) x[u] = reinterpret_cast<const float4*>(p.acc + part(head, s0 + SG * u) * HD)[d];
+#pragma unroll
+            for (int u = 0; u < MERGE_AHEAD; u++) {
+                if (s0 + SG * u >= S) continue;
+                const float f = sf[at][s0 + SG * u];
+                if (f == 0.0f) continue; /* a part without a sum has no values */
+                o.x = fmaf(x[u].x, f, o.x); o.y = fmaf(x[u].y, f, o.y); o.z = fmaf(x[u].z, f, o.z); o.w = fmaf(x[u].w, f, o.w);
             }
         }
-        reinterpret_cast<float4*>(a.out + (size_t)row * a.out_stride + (size_t)h * G * HD)[i] = o;
     }
+    if constexpr (SG > 1) {
+        so[tid] = o;
+        __syncthreads();
+        if (sg) return;
+#pragma unroll
+        for (int g = 1; g < SG; g++) {
+            const float4 x = so[tid + D * g];
+            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        }
+    }
+    if (head < a.n_heads) reinterpret_cast<float4*>(a.out + (size_t)row * a.out_stride + (size_t)head * HD)[d] = o;
 }
 
 /* How a call is cut into blocks. */
@@ -753,7 +816,13 @@ static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_
     } else {
         attend_own_kernel<HD, T><<<dim3(a.n * heads, p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
     }
-    if (p.own + p.tile > 1) attend_merge_kernel<HD><<<a.n * heads, 256, 0, s>>>(a, p);
+    const int S = p.own + p.tile;
+    if (S > 1) {
+        constexpr int at_once = 1024 / HD; /* heads a block of one thread for each four dimensions */
+        const auto blocks = [&](int sg) { return (unsigned)a.n * ((a.n_heads + at_once / sg - 1) / (at_once / sg)); };
+        if (S <= MERGE_AHEAD) attend_merge_kernel<HD, 1><<<blocks(1), 256, 0, s>>>(a, p);
+        else attend_merge_kernel<HD, 8><<<blocks(8), 256, 0, s>>>(a, p);
+    }
     return hipGetLastError();
 }
 

@@ -71,6 +71,8 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static size_t elem_bytes(int dtype) { return dtype == VITNA_DTYPE_F32 ? 4 : dtype == VITNA_DTYPE_F16 || dtype == VITNA_DTYPE_BF16 ? 2 : 0; }
 
 #define POSITIONS_MAX ((size_t)1 << 30)
+/* 64 positions lie within 2^31 bytes, so that kernels reach them with 32-bit offsets */
+#define POS_STRIDE_MAX ((size_t)1 << 23)
 /* no element of a view lies this far behind its start, so that offsets in bytes stay within 63 bits */
 #define EXTENT_MAX ((size_t)1 << 58)
 
@@ -93,6 +95,7 @@ static bool check_view(const vitna_hip_kv_view_t* c, char* err, size_t err_len) 
     if (c->seq_stride % lane || c->pos_stride % lane || c->head_stride % lane)
         return fail(err, err_len, "strides of %zu, %zu and %zu elements; whole multiples of %zu (16 bytes) are read", c->seq_stride, c->pos_stride,
                     c->head_stride, lane);
+    if (c->pos_stride > POS_STRIDE_MAX) return fail(err, err_len, "positions %zu elements apart; at most %zu are read", c->pos_stride, POS_STRIDE_MAX);
     if (!aligned16(c->k) || !aligned16(c->v)) return fail(err, err_len, "the keys and values have to be 16-byte aligned");
     size_t far = c->head_dim;
     if (!extend(c->seqs, c->seq_stride, &far) || !extend(c->ctx, c->pos_stride, &far) || !extend(c->n_kv_heads, c->head_stride, &far))
