@@ -8,11 +8,11 @@
  * with a running maximum and sum, both and the weighted values in float32 (the scores in units of log 2, so that
  * exp is exp2). Two kinds of block take parts of it:
  *
- *   own_part   a row's own positions (or all of them), for the G query heads of one key-value head: every position it
- *              loads is seen by all its columns. Bound by the cache's bytes; products on v_mfma_f32_16x16x4_f32.
- *   tile_part  positions that many rows see (a shared prefix, a prompt's chunk): 32 columns (row, query head) a wave,
- *              64 positions at a time through LDS, read once for all the block's columns. Products on
- *              v_mfma_f32_32x32x16_f16.
+ *   columns_part  up to 32 columns (row, query head) of one key-value head: a row's own positions, or a prefix that a few
+ *                 rows share. Each wave takes other positions, straight to registers. Bound by the cache's bytes;
+ *                 products on v_mfma_f32_16x16x4_f32.
+ *   tile_part     positions that many columns see (a shared prefix, a prompt's chunk): 32 columns a wave, 64 positions at a
+ *                 time through LDS, read once for all the block's columns. Products on v_mfma_f32_32x32x16_f16.
  *
  * Where a row's positions are split over several blocks, each leaves its maximum, sum and weighted values, and
  * attend_merge_kernel joins them.
@@ -67,7 +67,7 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-/* ---- a row's own positions ---- */
+/* ---- few columns: each wave other positions ---- */
 
 /* Dimension of element j of lane column c: pieces of 16 bytes (f16 heads of 64: 8), a wave's load whole rows. */
 template <int HD, typename T>
@@ -85,42 +85,49 @@ struct own_step {
     vec<T, own_dims<HD, T>::PE> v[4][own_dims<HD, T>::NP];
 };
 
-template <int HD, typename T, int NW>
-__device__ __forceinline__ void own_part(const attend_args& a, const attend_parts& p, int split, int h, int row, char* lds) {
+/* What columns_part reads: positions begin .. begin + n_sink - 1, then from .. , numbered 0, 1, ...; of them i0 .. i1 - 1.
+   Positions before shared lie `other` elements behind the cache's start, the rest `mine`. */
+struct positions {
+    int begin, n_sink, from, i0, i1, shared;
+    size_t other, mine;
+};
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) << 1; }
+#define MAG_INF 0xff000000u /* a magnitude that is no number's: the sign shifted out, a NaN is the largest, then an infinity */
+
+/* n_cols columns (16 at most) of key-value head h from col0 on (column x: row row0 + x / G, query head h G + x mod G), each
+   wave 16 positions a step, then the waves joined in LDS ([NW][16] maxima and sums, [NW][16][HD] values). MASK: a column
+   sees what its row (rows[x / G]) shares and its window leaves; otherwise all. Whole block; ends with LDS read. */
+template <int HD, typename T, int NW, bool MASK>
+__device__ __forceinline__ void columns_part(const attend_args& a, const attend_parts& p, const positions& at, int split, int h, int row0,
+                                             const attend_row* rows, int col0, int n_cols, char* lds) {
     constexpr int DPL = own_dims<HD, T>::DPL, PE = own_dims<HD, T>::PE, NP = own_dims<HD, T>::NP, STEP = 16 * NW;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c16 = lane & 15, kq = lane >> 4, G = a.n_heads / a.n_kv;
-    const attend_row r = row_of(a, row);
-    const int end = r.pos + 1, begin = p.tile ? min(r.shared, end) : 0;
-    /* seen: [begin, sink) and [from, end) */
-    const int sink = a.window ? max(begin, min(a.sinks, end)) : begin, from = a.window ? max(sink, end - a.window) : begin;
-    const int n_sink = sink - begin, count = n_sink + (end - from);
-    const int per = ((count + p.own - 1) / p.own + STEP - 1) / STEP * STEP;
-    const int i0 = (int)min((long)split * per, (long)count), i1 = min(i0 + per, count);
-    const int S = p.own + p.tile;
-    const size_t part = ((size_t)row * a.n_kv + h) * S + split;
+    const int S = p.own + p.tile, i0 = at.i0, i1 = at.i1;
     const bool direct = S == 1;
+    auto part_of = [&](int c) { const int col = col0 + c; return (((size_t)(row0 + col / G) * a.n_kv + h) * S + split) * G + col % G; };
+    auto out_of = [&](int c) { const int col = col0 + c; return a.out + (size_t)(row0 + col / G) * a.out_stride + (size_t)(h * G + col % G) * HD; };
     if (i0 >= i1) {
         if (!direct) {
-            if (tid < G) p.ml[part * G + tid] = make_float2(-INFINITY, 0.0f);
+            if (tid < n_cols) p.ml[part_of(tid)] = make_float2(-INFINITY, 0.0f);
         } else {
-            for (int i = tid; i < G * HD / 4; i += 64 * NW)
-                reinterpret_cast<float4*>(a.out + (size_t)row * a.out_stride + (size_t)h * G * HD)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = tid; i < n_cols * HD / 4; i += 64 * NW) reinterpret_cast<float4*>(out_of(i / (HD / 4)))[i % (HD / 4)] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         return;
     }
     const T* kc = (const T*)a.k + (size_t)h * a.head_stride;
     const T* vc = (const T*)a.v + (size_t)h * a.head_stride;
-    const size_t mine = (size_t)r.seq * a.seq_stride, other = (size_t)r.base * a.seq_stride;
+    auto position = [&](int i) { return i < at.n_sink ? at.begin + i : at.from + (i - at.n_sink); };
     auto place = [&](int i) {
-        const int t = i < n_sink ? begin + i : from + (i - n_sink);
-        return (t < r.shared ? other : mine) + (size_t)t * a.pos_stride;
+        const int t = position(i);
+        return (t < at.shared ? at.other : at.mine) + (size_t)t * a.pos_stride;
     };
     auto load = [&](int ib, own_step<HD, T>& s) {
         const int ik = ib + 16 * wave + c16;
         if (ik < i1) {
-            const T* at = kc + place(ik) + 8 * kq;
+            const T* k = kc + place(ik) + 8 * kq;
 #pragma unroll
-            for (int t = 0; t < HD / 32; t++) s.k[t] = *reinterpret_cast<const vec<T, 8>*>(at + 32 * t);
+            for (int t = 0; t < HD / 32; t++) s.k[t] = *reinterpret_cast<const vec<T, 8>*>(k + 32 * t);
         } else {
 #pragma unroll
             for (int t = 0; t < HD / 32; t++) s.k[t] = vec<T, 8>{};
@@ -129,9 +136,9 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
         for (int x = 0; x < 4; x++) {
             const int iv = ib + 16 * wave + 4 * kq + x;
             if (iv < i1) {
-                const T* at = vc + place(iv) + PE * c16;
+                const T* v = vc + place(iv) + PE * c16;
 #pragma unroll
-                for (int n = 0; n < NP; n++) s.v[x][n] = *reinterpret_cast<const vec<T, PE>*>(at + 64 * n);
+                for (int n = 0; n < NP; n++) s.v[x][n] = *reinterpret_cast<const vec<T, PE>*>(v + 64 * n);
             } else {
 #pragma unroll
                 for (int n = 0; n < NP; n++) s.v[x][n] = vec<T, PE>{};
@@ -140,16 +147,25 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
     };
     own_step<HD, T> cur, nxt;
     load(i0, cur);
-    /* head c16's query in units of log 2: B operand of step (t, m), dimension 32 t + 8 kq + m */
+    /* the queries in units of log 2: B operand of step (t, m), dimension 32 t + 8 kq + m of column 16 ct + c16 */
     float q[HD / 32][8];
+    int last = INT32_MAX, low = INT32_MIN;
     const float qs = a.scale * 1.44269504088896340736f;
+    {
+        const int col = col0 + min(c16, n_cols - 1), lr = col / G;
 #pragma unroll
-    for (int t = 0; t < HD / 32; t++) {
-        const float4* at = reinterpret_cast<const float4*>(a.q + (size_t)row * a.q_stride + (size_t)(h * G + min(c16, G - 1)) * HD + 32 * t + 8 * kq);
-        const float4 x = at[0], y = at[1];
-        const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        for (int t = 0; t < HD / 32; t++) {
+            const float4* src = reinterpret_cast<const float4*>(a.q + (size_t)(row0 + lr) * a.q_stride + (size_t)(h * G + col - lr * G) * HD + 32 * t + 8 * kq);
+            const float4 x = src[0], y = src[1];
+            const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int m = 0; m < 8; m++) q[t][m] = c16 < G ? w[m] * qs : 0.0f;
+            for (int m = 0; m < 8; m++) q[t][m] = c16 < n_cols ? w[m] * qs : 0.0f;
+        }
+        if constexpr (MASK) {
+            const attend_row r = rows[lr];
+            last = min(r.shared, r.pos + 1) - 1;
+            if (a.window) low = r.pos - a.window + 1;
+        }
     }
     float m_run = -INFINITY, l_run = 0.0f;
     f4v O[DPL];
@@ -157,79 +173,241 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
     for (int j = 0; j < DPL; j++) O[j] = f4v{0.f, 0.f, 0.f, 0.f};
     for (int ib = i0; ib < i1; ib += STEP) {
         if (ib + STEP < i1) load(ib + STEP, nxt);
-        /* S: positions 4 kq + x of head c16 */
-        f4v s[HD / 32];
+        const int mine = ib + 16 * wave + 4 * kq, left = i1 - mine; /* the lane's positions x < left are there */
+        uint32_t bad = 0; /* bit x: position 4 kq + x has values that are not finite */
+        if constexpr (MASK) {
+            uint32_t mag = 0;
 #pragma unroll
-        for (int t = 0; t < HD / 32; t++) {
-            s[t] = f4v{0.f, 0.f, 0.f, 0.f};
+            for (int x = 0; x < 4; x++)
 #pragma unroll
-            for (int m = 0; m < 8; m++) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)cur.k[t][m], q[t][m], s[t], 0, 0, 0);
+                for (int j = 0; j < DPL; j++) mag = max(mag, magnitude((float)cur.v[x][j / PE][j % PE]));
+            if (__builtin_expect(__any(mag >= MAG_INF), 0)) {
+                /* a weight of 0 would make NaN of them: taken out, and the columns that see one marked */
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    bool b = false;
+#pragma unroll
+                    for (int j = 0; j < DPL; j++)
+                        if (magnitude((float)cur.v[x][j / PE][j % PE]) >= MAG_INF) {
+                            cur.v[x][j / PE][j % PE] = (T)0.0f;
+                            b = true;
+                        }
+                    const uint64_t any = __ballot(b);
+                    if ((any >> (16 * kq)) & 0xffff) bad |= 1u << x;
+                }
+            }
         }
-        f4v S4 = s[0] + s[1];
-        if constexpr (HD == 128) S4 = S4 + (s[2] + s[3]);
-        const int left = i1 - (ib + 16 * wave + 4 * kq); /* the lane's positions x < left are there */
-        float m = m_run;
+        {
+            /* S: positions 4 kq + x of the column */
+            f4v s[HD / 32];
 #pragma unroll
-        for (int x = 0; x < 4; x++) m = fmaxf(m, x < left ? S4[x] : -INFINITY);
-        m = fmaxf(m, __shfl_xor(m, 16, WAVE));
-        m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-        const float base = m == -INFINITY ? 0.0f : m, f = exp2_hw(m_run - base);
-        float w[4], l = 0.0f;
+            for (int t = 0; t < HD / 32; t++) {
+                s[t] = f4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            w[x] = x < left ? exp2_hw(S4[x] - base) : 0.0f;
-            l += w[x];
+                for (int m = 0; m < 8; m++) s[t] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)cur.k[t][m], q[t][m], s[t], 0, 0, 0);
+            }
+            f4v S4 = s[0] + s[1];
+            if constexpr (HD == 128) S4 = S4 + (s[2] + s[3]);
+            bool sees[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                sees[x] = x < left;
+                if constexpr (MASK) {
+                    const int t = position(mine + x);
+                    sees[x] = sees[x] && t <= last && (t >= low || t < a.sinks);
+                }
+            }
+            float m = m_run;
+#pragma unroll
+            for (int x = 0; x < 4; x++) m = fmaxf(m, sees[x] ? S4[x] : -INFINITY);
+            m = fmaxf(m, __shfl_xor(m, 16, WAVE));
+            m = fmaxf(m, __shfl_xor(m, 32, WAVE));
+            const float base = m == -INFINITY ? 0.0f : m, f = exp2_hw(m_run - base);
+            float w[4], l = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                w[x] = sees[x] ? exp2_hw(S4[x] - base) : 0.0f;
+                l += w[x];
+                if constexpr (MASK)
+                    if (__builtin_expect(bad >> x & 1, 0) && sees[x]) l = NAN;
+            }
+            l_run = fmaf(l_run, f, l);
+            m_run = m;
+            if (__any(f != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < DPL; j++) O[j] = O[j] * f;
+            }
+            /* O^T: element 4 kq + i of piece dimensions, column c16 */
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+#pragma unroll
+                for (int j = 0; j < DPL; j++)
+                    O[j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)cur.v[x][j / PE][j % PE], w[x], O[j], 0, 0, 0);
         }
-        l_run = fmaf(l_run, f, l);
-        m_run = m;
-        if (__any(f != 1.0f)) {
-#pragma unroll
-            for (int j = 0; j < DPL; j++) O[j] = O[j] * f;
-        }
-        /* O^T: element 4 kq + i of piece dimensions, head c16 */
-#pragma unroll
-        for (int x = 0; x < 4; x++)
-#pragma unroll
-            for (int j = 0; j < DPL; j++) O[j] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)cur.v[x][j / PE][j % PE], w[x], O[j], 0, 0, 0);
         cur = nxt;
     }
-    l_run += __shfl_xor(l_run, 16, WAVE);
-    l_run += __shfl_xor(l_run, 32, WAVE);
-    /* the waves joined: m and l [NW][16], then the values [NW][G][HD] */
     float* wm = reinterpret_cast<float*>(lds);
     float* wl = wm + NW * 16;
     float* wacc = wl + NW * 16;
+    l_run += __shfl_xor(l_run, 16, WAVE);
+    l_run += __shfl_xor(l_run, 32, WAVE);
     if (kq == 0) {
         wm[wave * 16 + c16] = m_run;
         wl[wave * 16 + c16] = l_run;
     }
-    if (c16 < G) {
+    if (c16 < n_cols) {
 #pragma unroll
         for (int j = 0; j < DPL; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) wacc[(wave * G + c16) * HD + 64 * (j / PE) + PE * (4 * kq + i) + j % PE] = O[j][i];
+            for (int i = 0; i < 4; i++) wacc[(wave * n_cols + c16) * HD + 64 * (j / PE) + PE * (4 * kq + i) + j % PE] = O[j][i];
     }
     __syncthreads();
-    for (int i = tid; i < G * HD / 4; i += 64 * NW) {
-        const int g = i / (HD / 4), d = i % (HD / 4);
+    for (int i = tid; i < n_cols * HD / 4; i += 64 * NW) {
+        const int c = i / (HD / 4), d = i % (HD / 4);
         float M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w * 16 + g]);
+        for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w * 16 + c]);
         const float base = M == -INFINITY ? 0.0f : M;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float f = exp2_hw(wm[w * 16 + g] - base);
-            const float4 x = reinterpret_cast<const float4*>(wacc + (w * G + g) * HD)[d];
-            L = fmaf(wl[w * 16 + g], f, L);
+            const float f = exp2_hw(wm[w * 16 + c] - base);
+            const float4 x = reinterpret_cast<const float4*>(wacc + (w * n_cols + c) * HD)[d];
+            L = fmaf(wl[w * 16 + c], f, L);
             o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
         }
         if (direct) {
             const float inv = 1.0f / L;
-            reinterpret_cast<float4*>(a.out + (size_t)row * a.out_stride + (size_t)h * G * HD)[i] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            reinterpret_cast<float4*>(out_of(c))[d] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         } else {
-            reinterpret_cast<float4*>(p.acc + (part * G + g) * HD)[d] = o;
-            if (d == 0) p.ml[part * G + g] = make_float2(M, L);
+            const size_t part = part_of(c);
+            reinterpret_cast<float4*>(p.acc + part * HD)[d] = o;
+            if (d == 0) p.ml[part] = make_float2(M, L);
+        }
+    }
+}
+template <int HD, int NW>
+constexpr size_t columns_lds = NW * (32 + 16 * HD) * 4;
+
+/* A row's own positions, those that its window leaves. */
+template <int HD, typename T, int NW>
+__device__ __forceinline__ void own_part(const attend_args& a, const attend_parts& p, int split, int h, int row, char* lds) {
+    const attend_row r = row_of(a, row);
+    const int end = r.pos + 1, begin = p.tile ? min(r.shared, end) : 0;
+    /* seen: [begin, sink) and [from, end) */
+    const int sink = a.window ? max(begin, min(a.sinks, end)) : begin, from = a.window ? max(sink, end - a.window) : begin;
+    const int count = sink - begin + (end - from), per = ((count + p.own - 1) / p.own + 16 * NW - 1) / (16 * NW) * (16 * NW);
+    positions at;
+    at.begin = begin; at.n_sink = sink - begin; at.from = from;
+    at.i0 = (int)min((long)split * per, (long)count);
+    at.i1 = min(at.i0 + per, count);
+    at.shared = r.shared;
+    at.other = (size_t)r.base * a.seq_stride;
+    at.mine = (size_t)r.seq * a.seq_stride;
+    columns_part<HD, T, NW, false>(a, p, at, split, h, row, nullptr, 0, a.n_heads / a.n_kv, lds);
+}
+
+/* ---- rows that share ---- */
+
+#define FEW_COLUMNS 32 /* a group with so many columns at most goes to few_part, any other to tile_part */
+
+template <int HD>
+constexpr int tile_waves = HD == 128 ? 8 : 4;
+/* Rows of a tile. Rows next to each other in a tile that read the same positions of the same sequence are a group. */
+template <int HD>
+__host__ __device__ constexpr int tile_rows(int G) { return 32 * tile_waves<HD> / G; }
+
+/* A tile's rows to LDS (the caller waits). */
+template <int NT>
+__device__ __forceinline__ void load_rows(const attend_args& a, int r0, int nr, attend_row* srow) {
+    for (int i = threadIdx.x; i < nr; i += NT) srow[i] = row_of(a, r0 + i);
+}
+/* The row behind the group that begins at row first of the tile's nr. */
+__device__ __forceinline__ int group_end(const attend_row* srow, int first, int nr) {
+    const int lane = threadIdx.x & 63;
+    for (int w = first >> 6; w <= (nr - 1) >> 6; w++) {
+        const int i = 64 * w + lane;
+        bool starts = false;
+        if (i > first && i < nr) starts = srow[i].base != srow[i - 1].base || srow[i].shared != srow[i - 1].shared;
+        const uint64_t mask = __ballot(starts);
+        if (mask) return 64 * w + (int)__builtin_ctzll(mask);
+    }
+    return nr;
+}
+/* What some rows first .. next - 1 of a group see: [0, sink) and [from, end) of sequence seq. */
+struct group_span {
+    int seq, sink, from, end;
+};
+template <bool RUN>
+__device__ __forceinline__ group_span group_seen(const attend_args& a, const attend_row* srow, int first, int next) {
+    group_span s;
+    s.seq = __builtin_amdgcn_readfirstlane(RUN ? (a.rows ? srow[first].seq : a.run_seq) : srow[first].base);
+    int end = __builtin_amdgcn_readfirstlane(srow[first].shared), least = 0;
+    if (RUN || a.window) {
+        /* the rows' furthest and nearest positions */
+        uint32_t far = 0, near = 0; /* pos + 1, and 2^31 - pos: both maxima */
+        for (int i = first + (threadIdx.x & 63); i < next; i += 64) {
+            const int pos = srow[i].pos;
+            if (pos >= 0) {
+                far = max(far, (uint32_t)pos + 1);
+                near = max(near, 0x80000000u - (uint32_t)pos);
+            }
+        }
+        far = wave_umax(far);
+        near = wave_umax(near);
+        end = RUN ? (int)far : min(end, (int)far);
+        least = near ? (int)(0x80000000u - near) : 0;
+    }
+    s.end = min(end, a.ctx);
+    s.sink = a.window ? min(a.sinks, s.end) : 0;
+    s.from = a.window ? min(max(s.sink, least - a.window + 1), s.end) : 0;
+    return s;
+}
+
+/* The prefixes of a tile's groups of few columns. A unit is 16 columns of such a group; split x of the tile's p.tile takes
+   unit x mod (number of units), and of its positions part x / (number of units): one unit a block (as long as there are
+   splits enough), its part a long one. The other units' columns have nothing in split x. */
+template <int HD, typename T, int NW>
+__device__ __forceinline__ void few_part(const attend_args& a, const attend_parts& p, int split, int h, int tile, char* lds) {
+    const int G = a.n_heads / a.n_kv, TR = tile_rows<HD>(G), r0 = tile * TR, nr = min(TR, a.n - r0), tid = threadIdx.x, S = p.own + p.tile;
+    attend_row* srow = reinterpret_cast<attend_row*>(lds);
+    char* rest = lds + tile_rows<HD>(1) * sizeof(attend_row);
+    load_rows<64 * NW>(a, r0, nr, srow);
+    lds_barrier();
+    int units = 0;
+    for (int first = 0, next; first < nr; first = next) {
+        next = group_end(srow, first, nr);
+        const int n_cols = (next - first) * G;
+        if (n_cols <= FEW_COLUMNS) units += (n_cols + 15) >> 4;
+    }
+    if (!units) return;
+    const int parts = max(p.tile / units, 1); /* of a unit's positions */
+    int unit = 0;
+    for (int first = 0, next; first < nr; first = next) {
+        next = group_end(srow, first, nr);
+        const int n_cols = (next - first) * G;
+        if (n_cols > FEW_COLUMNS) continue;
+        for (int col = 0; col < n_cols; col += 16, unit++) {
+            const int many = min(16, n_cols - col);
+            /* with more units than splits each split takes every p.tile-th */
+            const bool mine = units <= p.tile ? split % units == unit && split / units < parts : unit % p.tile == split;
+            if (!mine) {
+                if (tid < many) {
+                    const int c = col + tid;
+                    p.ml[(((size_t)(r0 + first + c / G) * a.n_kv + h) * S + p.own + split) * G + c % G] = make_float2(-INFINITY, 0.0f);
+                }
+                continue;
+            }
+            const group_span s = group_seen<false>(a, srow, first, next);
+            const int count = s.sink + (s.end - s.from), per = ((count + parts - 1) / parts + 15) & ~15;
+            positions at;
+            at.begin = 0; at.n_sink = s.sink; at.from = s.from;
+            at.i0 = (int)min((long)(units <= p.tile ? split / units : 0) * per, (long)count);
+            at.i1 = min(at.i0 + per, count);
+            at.shared = INT32_MAX;
+            at.other = at.mine = (size_t)s.seq * a.seq_stride;
+            columns_part<HD, T, NW, true>(a, p, at, p.own + split, h, r0 + first, srow + first, col, many, rest);
+            lds_barrier();
         }
     }
 }
@@ -252,9 +430,6 @@ __device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, uin
                     pack_cut(fmaf(half_lo(hi.y), -1.0f, x2), fmaf(half_hi(hi.y), -1.0f, x3)));
 }
 
-/* Values as keys for a maximum of magnitudes: the sign shifted out, so a NaN is the largest, then an infinity. */
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) << 1; }
-#define MAG_INF 0xff000000u
 /* The k of 2^k that brings a magnitude to 2^14 .. 2^15 (0 and numbers near it: as far as 2^k reaches). */
 __device__ __forceinline__ int to_half_range(uint32_t mag) { return min(141 - (int)(mag >> 24), 126); }
 __device__ __forceinline__ float two_to(int k) { return __int_as_float((k + 127) << 23); } /* -126 .. 127 */
@@ -266,66 +441,104 @@ struct tile_shape {
     static constexpr int NT = 64 * NW, CC = HD / 4, U = 16 * CC / NT;    /* a thread's groups of 4 positions x 4 dimensions */
     static constexpr int HALF = 64 * HD;                                 /* values of one part of 64 positions' keys */
     static constexpr int ROWS = 32 * NW;                                 /* the most rows of a tile */
-    static constexpr size_t LDS = (PARTS ? 4 : 2) * HALF * 2 + ROWS * sizeof(attend_row) + 2 * NW * 4 + 8;
+    static constexpr size_t HEAD = (2 * NW * 4 + 8 + 15) / 16 * 16, LDS = ROWS * sizeof(attend_row) + HEAD + (PARTS ? 4 : 2) * HALF * 2;
+    static_assert(NW * 4096 <= (PARTS ? 4 : 2) * HALF * 2, "the queries pass through the keys' and values' room");
     static_assert(U >= 1 && U * NT == 16 * CC, "whole groups a thread");
 };
 
-/* RUN: the rows are tokens of one sequence, each seeing up to itself; otherwise each sees its shared prefix. */
+/* Split split of what the columns of rows row0 + 0 .. n_rows - 1 see together: RUN, rows of one sequence, each up to itself;
+   otherwise a group's shared prefix. srow are the rows. */
 template <int HD, typename T, int NW, bool RUN>
-__device__ __forceinline__ void tile_part(const attend_args& a, const attend_parts& p, int split, int h, int tile, char* lds) {
+__device__ __forceinline__ void group_part(const attend_args& a, const attend_parts& p, int split, int h, int row0, int n_rows,
+                                           const attend_row* srow, const group_span& s_, char* lds) {
     typedef tile_shape<HD, T, NW> sh;
     constexpr bool PARTS = sh::PARTS, SCALED = sh::SCALED;
     constexpr int KS = HD / 16, DT = HD / 32, U = sh::U, CC = sh::CC, HALF = sh::HALF;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c32 = lane & 31, hh = lane >> 5;
-    const int G = a.n_heads / a.n_kv, TR = 32 * NW / G, r0 = tile * TR, nr = min(TR, a.n - r0);
+    const int G = a.n_heads / a.n_kv, S = p.own + p.tile;
     /* Keys [part][64 positions][HD] in pieces of 8 dimensions, piece x of position t at x ^ t mod (HD / 8). Values
        [part][HD][64 positions] in units of two pieces of 4 positions, those of one MFMA operand (positions 16 s + 4 hh ..
        and 16 s + 8 + 4 hh ..: unit 2 s + hh), unit x of dimension d at x ^ (d / 2 ^ d / 16) mod 8. Sixteen lanes'
        16-byte reads then take every bank once, and all places are one lane's ^ and + a constant. */
-    char* sk = lds;
+    uint32_t* smax = reinterpret_cast<uint32_t*>(lds); /* [2][NW]: magnitudes of keys, of values */
+    uint32_t* sbad = smax + 2 * NW;                    /* positions whose values are not finite */
+    char* sk = lds + sh::HEAD;
     char* sv = sk + (PARTS ? 2 : 1) * HALF * 2;
-    attend_row* srow = reinterpret_cast<attend_row*>(sv + (PARTS ? 2 : 1) * HALF * 2);
     auto key_to = [&](int pg, int cc) { return (uint32_t)(4 * pg * HD * 2 + (((cc >> 1) ^ ((4 * pg) & (HD / 8 - 1))) << 4) + 8 * (cc & 1)); };
     auto value_to = [&](int pg, int cc) {
         const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1;
         return (uint32_t)(4 * cc * 128 + ((unit ^ (((2 * cc) ^ (cc >> 2)) & 7)) << 4) + 8 * half);
     };
-    uint32_t* smax = reinterpret_cast<uint32_t*>(srow + sh::ROWS); /* [2][NW]: magnitudes of keys, of values */
-    uint32_t* sbad = smax + 2 * NW;                        /* positions whose values are not finite */
 
-    for (int i = tid; i < nr; i += sh::NT) srow[i] = row_of(a, r0 + i);
-    if (tid < 2) sbad[tid] = 0;
-    lds_barrier();
-
+    /* seen, in chunks of 64 */
+    const int seq = s_.seq, sink = s_.sink, from = s_.from, end = s_.end;
+    const int n_sink = (sink + 63) >> 6, n_chunks = n_sink + ((end - from + 63) >> 6);
+    const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
     /* the lane's column */
     const int col = 32 * wave + c32, lr = col / G, g = col - lr * G;
-    const bool there = lr < nr;
+    const bool there = lr < n_rows;
     const attend_row me = srow[there ? lr : 0];
     const int last = !there ? -1 : RUN ? me.pos : min(me.shared, me.pos + 1) - 1; /* the last position it may see here */
     const int low = a.window ? me.pos - a.window + 1 : INT32_MIN;
+    const size_t row = (size_t)(row0 + lr), part = ((row * a.n_kv + h) * S + p.own + split) * G + g;
+    if (c0 >= c1) {
+        if (!there || hh) return;
+        if (S > 1) p.ml[part] = make_float2(-INFINITY, 0.0f);
+        else
+            for (int i = 0; i < HD / 4; i++) reinterpret_cast<float4*>(a.out + row * a.out_stride + (size_t)(h * G + g) * HD)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        return;
+    }
+    if (tid < 2) sbad[tid] = 0;
     h8v qh[KS], ql[KS];
     float to_score; /* from the products' sums to scores in units of log 2, with the keys' power of two */
     {
-        const float* at = a.q + (size_t)(r0 + (there ? lr : 0)) * a.q_stride + (size_t)(h * G + g) * HD + 8 * hh;
-        /* read twice: kept between, the values would take the registers that the loop needs */
+        /* The wave's 32 columns through 4 KB of LDS of its own, 32 dimensions at a time: loaded 128 bytes a column (a lane
+           a column would ask for 64 lines an instruction, 18000 cycles a block), taken as operand 16 s + 8 hh .. */
+        float4 in[KS / 2][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = 32 * wave + 8 * i + (lane >> 3), r = min(c / G, n_rows - 1);
+            const float* from_ = a.q + (size_t)(row0 + r) * a.q_stride + (size_t)(h * G + c % G) * HD + 4 * (lane & 7);
+#pragma unroll
+            for (int t = 0; t < KS / 2; t++) in[t][i] = *reinterpret_cast<const float4*>(from_ + 32 * t);
+        }
+        /* a column's largest magnitude, from its eight lanes to its two */
         uint32_t mag = 0;
 #pragma unroll
-        for (int s = 0; s < 2 * KS; s++) {
-            const float4 x = *reinterpret_cast<const float4*>(at + 16 * (s >> 1) + 4 * (s & 1));
-            mag = max(max(mag, max(magnitude(x.x), magnitude(x.y))), max(magnitude(x.z), magnitude(x.w)));
+        for (int i = 0; i < 4; i++) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int t = 0; t < KS / 2; t++) most = max(max(most, max(magnitude(in[t][i].x), magnitude(in[t][i].y))), max(magnitude(in[t][i].z), magnitude(in[t][i].w)));
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d, WAVE));
+            most = (uint32_t)__shfl((int)most, 8 * (c32 & 7), WAVE);
+            if ((c32 >> 3) == i) mag = most;
         }
-        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32, WAVE));
         const int k = to_half_range(mag);
         const float f = two_to(k);
         to_score = a.scale * 1.44269504088896340736f * two_to(-k);
+        char* mine = sk + wave * 4096;
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const float4 x = *reinterpret_cast<const float4*>(at + 16 * s), y = *reinterpret_cast<const float4*>(at + 16 * s + 4);
-            uint2 h0, l0, h1, l1;
-            cut4(x.x, x.y, x.z, x.w, f, h0, l0);
-            cut4(y.x, y.y, y.z, y.w, f, h1, l1);
-            qh[s] = __builtin_bit_cast(h8v, u32x4{h0.x, h0.y, h1.x, h1.y});
-            ql[s] = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
+        for (int t = 0; t < KS / 2; t++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int c = 8 * i + (lane >> 3);
+                *reinterpret_cast<float4*>(mine + c * 128 + (((lane & 7) ^ (c & 7)) << 4)) = in[t][i];
+            }
+            __builtin_amdgcn_wave_barrier(); /* LDS operations of one wave complete in order */
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const float4 x = *reinterpret_cast<const float4*>(mine + c32 * 128 + (((4 * s + 2 * hh) ^ (c32 & 7)) << 4));
+                const float4 y = *reinterpret_cast<const float4*>(mine + c32 * 128 + (((4 * s + 2 * hh + 1) ^ (c32 & 7)) << 4));
+                uint2 h0, l0, h1, l1;
+                cut4(x.x, x.y, x.z, x.w, f, h0, l0);
+                cut4(y.x, y.y, y.z, y.w, f, h1, l1);
+                qh[2 * t + s] = __builtin_bit_cast(h8v, u32x4{h0.x, h0.y, h1.x, h1.y});
+                ql[2 * t + s] = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
     const char* key_at = sk + c32 * HD * 2;
@@ -343,51 +556,10 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
     const T* kh = (const T*)a.k + (size_t)h * a.head_stride;
     const T* vh = (const T*)a.v + (size_t)h * a.head_stride;
     const uint32_t pos_bytes = (uint32_t)(a.pos_stride * sizeof(T)); /* 64 of them stay within 31 bits */
-    int first = 0;
-    while (first < nr) {
-        /* rows first .. next - 1 read the same positions of the same sequence */
-        int next = nr;
-        if constexpr (!RUN) {
-            for (int w = first >> 6; w <= (nr - 1) >> 6; w++) {
-                const int i = 64 * w + lane;
-                bool starts = false;
-                if (i > first && i < nr) starts = srow[i].base != srow[i - 1].base || srow[i].shared != srow[i - 1].shared;
-                const uint64_t mask = __ballot(starts);
-                if (mask) {
-                    next = 64 * w + __builtin_ctzll(mask);
-                    break;
-                }
-            }
-        }
-        const int mine0 = first;
-        first = next;
-        const int seq = __builtin_amdgcn_readfirstlane(RUN ? (a.rows ? srow[mine0].seq : a.run_seq) : srow[mine0].base);
-        int end = __builtin_amdgcn_readfirstlane(srow[mine0].shared), least = 0;
-        if (RUN || a.window) {
-            /* the rows' furthest and nearest positions */
-            uint32_t far = 0, near = 0; /* pos + 1, and 2^31 - pos: both maxima */
-            for (int i = mine0 + lane; i < next; i += 64) {
-                const int pos = srow[i].pos;
-                if (pos >= 0) {
-                    far = max(far, (uint32_t)pos + 1);
-                    near = max(near, 0x80000000u - (uint32_t)pos);
-                }
-            }
-            far = wave_umax(far);
-            near = wave_umax(near);
-            end = RUN ? (int)far : min(end, (int)far);
-            least = near ? (int)(0x80000000u - near) : 0;
-        }
-        end = min(end, a.ctx);
-        /* seen by some row: [0, sink) and [from, end), in chunks of 64 */
-        const int sink = a.window ? min(a.sinks, end) : 0, from = a.window ? min(max(sink, least - a.window + 1), end) : 0;
-        const int n_sink = (sink + 63) >> 6, n_chunks = n_sink + ((end - from + 63) >> 6);
-        const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
-        if (c0 >= c1) continue;
-        const bool on = there && lr >= mine0 && lr < next && last >= 0;
-        const bool wave_on = __any(on);
-        const T* ks = kh + (size_t)seq * a.seq_stride;
-        const T* vs = vh + (size_t)seq * a.seq_stride;
+    const bool on = there && last >= 0, wave_on = __any(on);
+    const T* ks = kh + (size_t)seq * a.seq_stride;
+    const T* vs = vh + (size_t)seq * a.seq_stride;
+    {
         auto start = [&](int c) { return c < n_sink ? 64 * c : from + 64 * (c - n_sink); };
         auto stop = [&](int c) { return c < n_sink ? sink : end; };
         vec<T, 4> rk[U][4], rv[U][4];
@@ -627,20 +799,17 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
                 }
             }
         }
-        lds_barrier(); /* every wave is past the last chunk before another group's first */
     }
 
     l_run += __shfl_xor(l_run, 32, WAVE);
     if (!there) return;
-    const int S = p.own + p.tile;
     const float back = SCALED ? two_to(-e_out) : 1.0f;
     float* to;
     float f;
     if (S == 1) {
-        to = a.out + (size_t)(r0 + lr) * a.out_stride + (size_t)(h * G + g) * HD;
+        to = a.out + row * a.out_stride + (size_t)(h * G + g) * HD;
         f = l_run == 0.0f ? 0.0f : back / l_run;
     } else {
-        const size_t part = (((size_t)(r0 + lr) * a.n_kv + h) * S + p.own + split) * G + g;
         if (hh == 0) p.ml[part] = make_float2(m_run, l_run * 0x1p-14f);
         if (l_run == 0.0f) return;
         to = p.acc + part * HD;
@@ -653,42 +822,50 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
             *reinterpret_cast<float4*>(to + 32 * d + 8 * i + 4 * hh) = make_float4(O[d][4 * i] * f, O[d][4 * i + 1] * f, O[d][4 * i + 2] * f, O[d][4 * i + 3] * f);
 }
 
+/* Split split of a tile's rows: RUN all together, otherwise its groups of many columns, one after another. */
+template <int HD, typename T, int NW, bool RUN>
+__device__ __forceinline__ void tile_part(const attend_args& a, const attend_parts& p, int split, int h, int tile, char* lds) {
+    const int G = a.n_heads / a.n_kv, TR = tile_rows<HD>(G), r0 = tile * TR, nr = min(TR, a.n - r0);
+    attend_row* srow = reinterpret_cast<attend_row*>(lds);
+    char* rest = lds + tile_rows<HD>(1) * sizeof(attend_row);
+    load_rows<64 * NW>(a, r0, nr, srow);
+    lds_barrier();
+    if constexpr (RUN) {
+        group_part<HD, T, NW, true>(a, p, split, h, r0, nr, srow, group_seen<true>(a, srow, 0, nr), rest);
+    } else {
+        for (int first = 0, next; first < nr; first = next) {
+            next = group_end(srow, first, nr);
+            if ((next - first) * G <= FEW_COLUMNS) continue;
+            group_part<HD, T, NW, false>(a, p, split, h, r0 + first, next - first, srow + first, group_seen<false>(a, srow, first, next), rest);
+            lds_barrier();
+        }
+    }
+}
+
 /* ---- the kernels ---- */
 
-template <int HD>
-constexpr int tile_waves = HD == 128 ? 8 : 4;
 #define OWN_WAVES 4
 
+/* Rows' own parts alone: block (row, key-value head), split. */
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_own_kernel(attend_args a, attend_parts p) {
-    __shared__ __attribute__((aligned(16))) char lds[OWN_WAVES * (32 + ATTEND_G_MAX * HD) * 4];
+    __shared__ __attribute__((aligned(16))) char lds[columns_lds<HD, OWN_WAVES>];
     own_part<HD, T, OWN_WAVES>(a, p, blockIdx.y, blockIdx.x % a.n_kv, blockIdx.x / a.n_kv, lds);
 }
 
+/* The prefixes of groups of few columns, tile by tile, then the rows' own parts. */
 template <int HD, typename T>
-__global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_run_kernel(attend_args a, attend_parts p) {
-    __shared__ __attribute__((aligned(16))) char lds[tile_shape<HD, T, tile_waves<HD>>::LDS];
-    tile_part<HD, T, tile_waves<HD>, true>(a, p, blockIdx.y, blockIdx.x % a.n_kv, blockIdx.x / a.n_kv, lds);
+__global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(attend_args a, attend_parts p) {
+    __shared__ __attribute__((aligned(16))) char lds[columns_lds<HD, OWN_WAVES> + tile_rows<HD>(1) * sizeof(attend_row)];
+    const int tiles = p.tiles * a.n_kv * p.tile, b = (int)blockIdx.x < tiles ? blockIdx.x : blockIdx.x - tiles, h = b % a.n_kv, x = b / a.n_kv;
+    if ((int)blockIdx.x < tiles) few_part<HD, T, OWN_WAVES>(a, p, x % p.tile, h, x / p.tile, lds);
+    else own_part<HD, T, OWN_WAVES>(a, p, x % p.own, h, x / p.own, lds);
 }
 
-/* shared prefixes and the rows' own parts in one launch: the tiles' blocks first */
-template <int HD, typename T>
-__global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_shared_kernel(attend_args a, attend_parts p) {
-    constexpr int NW = tile_waves<HD>;
-    constexpr size_t A = tile_shape<HD, T, NW>::LDS, B = NW * (32 + ATTEND_G_MAX * HD) * 4;
-    __shared__ __attribute__((aligned(16))) char lds[A > B ? A : B];
-    const int tiles = p.tiles * a.n_kv * p.tile;
-    int b = blockIdx.x;
-    if (b < tiles) {
-        const int h = b % a.n_kv;
-        b /= a.n_kv;
-        tile_part<HD, T, NW, false>(a, p, b % p.tile, h, b / p.tile, lds);
-    } else {
-        b -= tiles;
-        const int h = b % a.n_kv;
-        b /= a.n_kv;
-        own_part<HD, T, NW>(a, p, b % p.own, h, b / p.own, lds);
-    }
+template <int HD, typename T, bool RUN>
+__global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_tile_kernel(attend_args a, attend_parts p) {
+    __shared__ __attribute__((aligned(16))) char lds[tile_shape<HD, T, tile_waves<HD>>::LDS];
+    tile_part<HD, T, tile_waves<HD>, RUN>(a, p, blockIdx.y, blockIdx.x % a.n_kv, blockIdx.x / a.n_kv, lds);
 }
 
 /* HB heads of a row a block, SG threads for each four dimensions of one: the parts' factors once in LDS, then each
@@ -786,11 +963,12 @@ static attend_parts plan(const attend_args& a) {
         return p;
     }
     if (a.shared_max) {
+        /* only groups of few columns: two of their blocks a compute unit */
         const long chunks = (a.window ? std::min<long>(a.shared_max, (long)a.window + a.sinks) : a.shared_max) / 64 + 1;
-        p.tile = (int)std::min<long>(std::min<long>(chunks, 64), std::max<long>(1, blocks / ((long)p.tiles * a.n_kv)));
+        const bool few = a.n * G <= FEW_COLUMNS;
+        p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), std::max<long>(1, (few ? 2 : 1) * blocks / ((long)p.tiles * a.n_kv)));
     }
-    const long step = 16 * (a.shared_max ? nw : OWN_WAVES);
-    p.own = (int)std::min<long>(std::min<long>((seen + step - 1) / step, 256), std::max<long>(1, 1024 / ((long)a.n * a.n_kv)));
+    p.own = (int)std::min<long>(std::min<long>((seen + 16 * OWN_WAVES - 1) / (16 * OWN_WAVES), 256), std::max<long>(1, 1024 / ((long)a.n * a.n_kv)));
     return p;
 }
 
@@ -810,9 +988,10 @@ static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_
     constexpr int NW = tile_waves<HD>;
     const unsigned heads = (unsigned)a.n_kv;
     if (a.run) {
-        attend_run_kernel<HD, T><<<dim3(p.tiles * heads, p.tile), 64 * NW, 0, s>>>(a, p);
+        attend_tile_kernel<HD, T, true><<<dim3(p.tiles * heads, p.tile), 64 * NW, 0, s>>>(a, p);
     } else if (p.tile) {
-        attend_shared_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.tile + (unsigned)a.n * p.own), 64 * NW, 0, s>>>(a, p);
+        attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.tile + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
+        if (a.n * (a.n_heads / a.n_kv) > FEW_COLUMNS) attend_tile_kernel<HD, T, false><<<dim3(p.tiles * heads, p.tile), 64 * NW, 0, s>>>(a, p);
     } else {
         attend_own_kernel<HD, T><<<dim3(a.n * heads, p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
     }
@@ -831,7 +1010,7 @@ hipError_t launch_attend(const attend_args& a, hipStream_t s) {
     attend_parts p = plan(a);
     size_t acc;
     if (parts_bytes(a, p, &acc) > a.work_bytes || p.own + p.tile > MERGE_SPLITS) return hipErrorInvalidValue;
-    if ((long)a.n * a.n_kv > INT32_MAX || (long)a.n_kv * ((long)p.tiles * p.tile + (long)a.n * p.own) > INT32_MAX) return hipErrorInvalidValue;
+    if ((long)a.n * a.n_kv > (1L << 22)) return hipErrorInvalidValue; /* threads of a launch stay within 32 bits */
     p.ml = static_cast<float2*>(a.work);
     p.acc = reinterpret_cast<float*>(static_cast<char*>(a.work) + acc);
     if (a.hd == 128) {
