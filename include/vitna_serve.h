@@ -122,6 +122,44 @@ bool vitna_hip_beam_select(const float* logits, size_t stride, size_t vocab, siz
 bool vitna_hip_kv_reorder(const vitna_hip_kv_view_t* c, size_t layers, size_t layer_stride, const int32_t* seqs, const int32_t* parents,
                           const int32_t* spans, size_t groups, size_t width, size_t longest, void* stream, char* err, size_t err_len);
 
+/* ---- the same on a model (vitna_cuda_create) ---- */
+
+/** A sliding window for every later step and pass of g: a row at position p
+    attends to positions p - window + 1 .. p and to the first sinks of its
+    sequence. window 0, or as long as the cache: none (as after
+    vitna_cuda_create). Every path honours it except the persistent step
+    kernel, whose steps then run the per-layer kernels. Passes of up to
+    vitna_hip_set_exact_rows rows still give each row the bits of its own
+    step. Keys and values behind the window stay in the cache. */
+bool vitna_hip_set_window(struct vitna_cuda_model* g, size_t window, size_t sinks, char* err, size_t err_len);
+
+/** The first n_pos positions of sequence src, every layer, copied into the n
+    sequences dst (distinct, none of them src), enqueued on the model's stream.
+    Until one of them changes such a position (a row or vitna_hip_kv at it),
+    rows steps (vitna_hip_moe_rows_step) whose rows of these sequences stand
+    next to each other read the positions once for all of them: the same
+    logits to the multi-row kernels' accuracy (two such passes lie within 4e-5
+    of max |logit| of each other), not the same bits. */
+bool vitna_hip_kv_fork(struct vitna_cuda_model* g, size_t src, size_t n_pos, const int32_t* dst, size_t n, char* err, size_t err_len);
+
+/** One step of beam search for groups prompts with width beams each
+    (groups x width rows, at most a pass's): the rows step of rows, the width
+    best continuations of each group (as vitna_hip_beam_select chooses them,
+    largest first), and the caches for the next step. rows[i] is beam i %
+    width of group i / width, each in a sequence of its own. On return rows
+    holds the continuations (token, position and the sequence that holds their
+    cache), scores their sums of log probabilities, ended whether their last
+    token was end_token (-1: there is none), parents (or NULL) the beam each
+    came from. The first continuation of a beam stays in its sequence; others
+    take the sequences of beams without one, whose positions behind the prefix
+    that the group shares (vitna_hip_kv_fork) are copied over. A beam that has
+    ended stays as it is, with its score. For a prompt's first step give its
+    last token to width sequences that hold the rest, and the scores 0, -inf,
+    -inf, ...: all continuations then come from the first. Where fewer than
+    width continuations remain, the rest have score -inf and parent -1. */
+bool vitna_hip_beam_step(struct vitna_cuda_model* g, vitna_cuda_row_t* rows, size_t groups, size_t width, float* scores, uint8_t* ended,
+                         int32_t end_token, int32_t* parents, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,10 +17,12 @@
  */
 
 #include "vitna_kernels.h"
+#include "serve_kernels.h"
 #include "step_kernel.h"
 #include "expert_cache.h"
 #include "host_copy.h"
 #include "../../include/vitna_hip.h"
+#include "../../include/vitna_serve.h"
 
 #include <stdarg.h>
 #include <stdio.h>
@@ -30,6 +32,7 @@
 #include <algorithm>
 #include <type_traits>
 #include <mutex>
+#include <new>
 
 /* The most rows a pass takes (the reference's MOE_ROWS, model_cuda.cu:197): model.c runs a prompt in chunks of
    this many. Scratch for this many rows is allocated with the model. */
@@ -63,6 +66,11 @@
 #define ROUTE_WIDE_ROWS 128
 /* rows step graphs kept at once: a prompt's passes take up to three attention grids, and a ragged step a fourth */
 #define ROWS_GRAPHS 4
+
+/* What a sequence shares: its first len positions are those of sequence base (both hold them). */
+struct seq_share {
+    int32_t base, len;
+};
 
 struct dlayer {
     qmat q, k, v, o;
@@ -142,6 +150,7 @@ struct vitna_cuda_model {
         int n;                  /* rows, or 0 for an empty entry */
         bool shared, one_seq;   /* two rows or more of one sequence; all of them (attention over tiles of rows) */
         bool fast;              /* the experts in 16-bit activations */
+        int prefix, own;        /* the attention over shared prefixes (rows_prefix, rows_own) */
         int splits;             /* the attention's grid */
         int head;               /* the head's rows: HEAD_ALL, HEAD_NONE or the one row */
         uint64_t used;
@@ -186,6 +195,21 @@ struct vitna_cuda_model {
     uint8_t* st_area[3];
     size_t st_stride[3];
     std::vector<int64_t> st_place;
+    /* attention with a window or over shared prefixes (launch_attend), and beam search: set up on first use */
+    int window, sinks;             /* window 0: none */
+    std::vector<seq_share> share;  /* of every sequence; empty until ensure_serve */
+    std::vector<int32_t> held;     /* of every sequence: no share reaches past this position of it */
+    bool sharing;                  /* some len is not 0 */
+    int2* share_dev;
+    seq_share* share_host;         /* pinned */
+    char* attend_buf;              /* launch_attend's scratch, for any pass */
+    size_t attend_bytes;
+    int rows_prefix, rows_own;     /* the pass's longest prefix that rows next to each other share, and its rows' longest part behind it (powers of two; 0: none shared) */
+    int32_t *fork_dev, *fork_host; /* a reordering's sequences, parents and spans; host pinned */
+    hipEvent_t serve_copied;       /* the last copies out of share_host, fork_host and beam_host have run */
+    char *beam_dev, *beam_host;    /* a beam step's scores and results ([ROWS_MAX] each; host pinned) */
+    char* beam_work;
+    size_t beam_work_bytes;
 };
 
 static bool fail(char* err, size_t len, const char* fmt, ...) {
@@ -518,6 +542,10 @@ extern "C" void vitna_cuda_free(struct vitna_cuda_model* g) {
     if (g->rows_copied) (void)hipEventDestroy(g->rows_copied);
     if (g->rt_host) (void)hipHostFree(g->rt_host);
     if (g->rt_copied) (void)hipEventDestroy(g->rt_copied);
+    if (g->share_host) (void)hipHostFree(g->share_host);
+    if (g->fork_host) (void)hipHostFree(g->fork_host);
+    if (g->beam_host) (void)hipHostFree(g->beam_host);
+    if (g->serve_copied) (void)hipEventDestroy(g->serve_copied);
     ec_destroy(g->ec);
     host_copy_destroy(g->results);
     if (g->stream) (void)hipStreamDestroy(g->stream);
@@ -703,6 +731,51 @@ extern "C" struct vitna_cuda_model* vitna_cuda_create(const vitna_llama_t* m, co
 
 /* ---- per-layer enqueues ---------------------------------------------- */
 
+/* The blocks a row's own part is split over in passes whose rows get the bits of their own steps: whatever the pass. */
+static int attend_splits(const vitna_cuda_model* g) {
+    const size_t seen = std::min((size_t)g->ctx, (size_t)g->window + g->sinks);
+    return (int)std::min<size_t>((seen + 63) / 64, 64);
+}
+
+/* launch_attend's view of layer's cache, the pass's rows in rows_dev and their queries, prepared, in qp. */
+static attend_args model_attend(const vitna_cuda_model* g, int layer, int n) {
+    attend_args t = {};
+    t.k = g->k_cache + (size_t)layer * g->layer_kv;
+    t.v = g->v_cache + (size_t)layer * g->layer_kv;
+    t.seq_stride = (size_t)g->NL * g->layer_kv;
+    t.pos_stride = (size_t)g->nkv * g->hd;
+    t.head_stride = g->hd;
+    t.dtype = VITNA_DTYPE_F32; t.n_heads = g->nh; t.n_kv = g->nkv; t.hd = g->hd; t.ctx = g->ctx; t.seqs = g->seqs;
+    t.window = g->window; t.sinks = g->sinks;
+    t.scale = 1.0f / sqrtf((float)g->hd);
+    t.q = g->qp; t.out = g->att;
+    t.q_stride = t.out_stride = (size_t)g->nh * g->hd;
+    t.n = n;
+    t.recs = g->rows_dev;
+    t.own_max = std::min(g->splits_grid * ATTN_CHUNK, g->ctx);
+    t.work = g->attend_buf; t.work_bytes = g->attend_bytes;
+    return t;
+}
+
+/* The pass's rows through the windowed attention (or over their shared prefixes): queries, keys and values of a are
+   prepared and stored first. exact: each row the bits of its own step. */
+static hipError_t enqueue_attend(vitna_cuda_model* g, int layer, attn_args a, bool exact) {
+    a.q_out = g->qp;
+    const hipError_t e = launch_attention_prepare(a, g->stream);
+    if (e != hipSuccess) return e;
+    attend_args t = model_attend(g, layer, a.n_rows);
+    if (exact) {
+        t.splits = attend_splits(g);
+    } else if (g->rows_one_seq && a.n_rows > 1) {
+        t.run = 1;
+    } else if (g->rows_prefix) {
+        t.share = g->share_dev;
+        t.shared_max = g->rows_prefix;
+        t.own_max = std::min(g->rows_own, g->ctx);
+    }
+    return launch_attend(t, g->stream);
+}
+
 /* One row's attention and o-projection. Where the layer takes the merged o-projection its parts stay pending
    (g->parts_n) for the router and the experts' down kernel, which add them to x; vitna_hip_residual adds them when
    the residual is read before that. */
@@ -736,16 +809,16 @@ static hipError_t enqueue_attention(vitna_cuda_model* g, int layer, int n_rows, 
     a.eps = g->eps;
     a.prepared = prepared ? 1 : 0;
     a.mma = 1;
-    e = launch_attention(a, g->stream);
-    if (e != hipSuccess) return e;
     g->parts_n = 0;
-    if (attention_oproj_fits(a, d.o)) {
+    e = g->window ? enqueue_attend(g, layer, a, true) : launch_attention(a, g->stream);
+    if (e != hipSuccess) return e;
+    if (!g->window && attention_oproj_fits(a, d.o)) {
         e = launch_attention_oproj(a, d.o, g->parts, g->stream);
         if (e != hipSuccess) return e;
         g->parts_n = g->nh / ATTN_OPROJ_HEADS;
         return hipSuccess;
     }
-    e = launch_attention_merge(a, g->stream);
+    if (!g->window) e = launch_attention_merge(a, g->stream);
     if (e != hipSuccess) return e;
     gemv_args go;
     memset(&go, 0, sizeof(go));
@@ -841,12 +914,16 @@ static int splits_bucket(const vitna_cuda_model* g, int max_pos) {
     return b < g->splits_max ? b : g->splits_max;
 }
 
+static void unshare(vitna_cuda_model* g, int seq, int from);
+static bool push_share(vitna_cuda_model* g, char* err, size_t err_len);
+
 static bool set_row(vitna_cuda_model* g, size_t seq, int32_t token, size_t pos, char* err, size_t err_len) {
     if (seq >= (size_t)g->seqs) return fail(err, err_len, "sequence %zu: the cache holds %d", seq, g->seqs);
     if (pos >= (size_t)g->ctx) return fail(err, err_len, "position %zu: the cache holds %d", pos, g->ctx);
     if (g->attention && (token < 0 || token >= g->V)) return fail(err, err_len, "token %d is outside the vocabulary of %d", token, g->V);
     const row_rec r = {token, (int32_t)pos, (int32_t)seq};
     g->splits_grid = splits_bucket(g, (int)pos);
+    if (g->sharing) unshare(g, (int)seq, (int)pos);
     /* the layers of one token after the first find their row in place */
     if (g->row_set && g->row_last.token == r.token && g->row_last.pos == r.pos && g->row_last.seq == r.seq) return true;
     /* the previous copy out of the page-locked row must have run */
@@ -1244,7 +1321,7 @@ static bool ensure_step(vitna_cuda_model* g, char* err, size_t err_len) {
 /* Whether this call runs the persistent step: asked for, and the model's shape takes it. */
 static bool use_step(vitna_cuda_model* g, bool* mega, char* err, size_t err_len) {
     *mega = false;
-    if (!g->step_want) return true;
+    if (!g->step_want || g->window) return true; /* its attention has no window */
     if (!ensure_step(g, err, err_len)) return false;
     *mega = g->step_state > 0;
     return true;
@@ -1362,6 +1439,7 @@ extern "C" bool vitna_hip_step_trace(struct vitna_cuda_model* g, size_t seq, int
     if (!g || g->lost) return fail(err, err_len, "the device model is not usable");
     if (!ensure_step(g, err, err_len)) return false;
     if (g->step_state < 1) return fail(err, err_len, "this model runs the per-layer kernels (%s)", g->step_reason);
+    if (g->window) return fail(err, err_len, "the persistent step has no window");
     if (block < 0 || block >= g->step_nb) return fail(err, err_len, "block %d: the step runs %d", block, g->step_nb);
     const size_t need = (size_t)g->NL * STEP_TRACE_PER_LAYER;
     if (n < need) return fail(err, err_len, "the timeline takes %zu words", need);
@@ -1512,6 +1590,7 @@ extern "C" bool vitna_hip_kv(struct vitna_cuda_model* g, size_t seq, size_t laye
     const size_t off = ((size_t)seq * g->NL + layer) * g->layer_kv + pos0 * kd;
     HIP_TRY(hipStreamSynchronize(g->stream), "waiting for the device");
     const hipMemcpyKind kind = write ? hipMemcpyHostToDevice : hipMemcpyDeviceToHost;
+    if (write && n && g->sharing) unshare(g, (int)seq, (int)pos0);
     if (k) HIP_TRY(write ? hipMemcpy(g->k_cache + off, k, n * kd * 4, kind) : hipMemcpy(k, g->k_cache + off, n * kd * 4, kind), "copying keys");
     if (v) HIP_TRY(write ? hipMemcpy(g->v_cache + off, v, n * kd * 4, kind) : hipMemcpy(v, g->v_cache + off, n * kd * 4, kind), "copying values");
     return true;
@@ -1522,6 +1601,7 @@ extern "C" bool vitna_hip_kv_fill(struct vitna_cuda_model* g, uint64_t seed, con
     const size_t kd = (size_t)g->nkv * g->hd;
     for (int s = 0; s < g->seqs; s++) {
         const size_t n = std::min(n_pos[s], (size_t)g->ctx);
+        if (n && g->sharing) unshare(g, s, 0);
         for (int l = 0; l < g->NL; l++) {
             const size_t off = ((size_t)s * g->NL + l) * g->layer_kv;
             const uint64_t tag = (seed * 1000003ull + (uint64_t)s) * 1000003ull + (uint64_t)l;
@@ -2131,6 +2211,13 @@ static hipError_t enqueue_rows_attention(vitna_cuda_model* g, int layer, int n, 
     a.eps = g->eps;
     /* several rows: the score and value products on the matrix cores */
     a.mma = n > 1 ? 1 : 0;
+    if (g->window || g->rows_prefix) {
+        e = enqueue_attend(g, layer, a, false);
+        gemv_multi_args go;
+        memset(&go, 0, sizeof(go));
+        go.w[0] = d.o; go.y[0] = g->x; go.nm = 1; go.x = g->att; go.n = n; go.xstride = g->nh * g->hd; go.add = 1;
+        return e == hipSuccess ? enqueue_multi(g, go, false) : e;
+    }
     if (g->rows_shared_seq) {
         /* rows of one sequence see each other's keys: all of them stored before any attention reads */
         a.q_out = g->qp;
@@ -2311,21 +2398,21 @@ static hipError_t enqueue_exact_attention(vitna_cuda_model* g, int layer, int n)
     a.splits_grid = g->splits_grid;
     a.eps = g->eps;
     a.mma = 1;
-    if (g->rows_shared_seq) {
+    if (!g->window && g->rows_shared_seq) {
         a.q_out = g->qp;
         e = launch_attention_prepare(a, g->stream);
         if (e != hipSuccess) return e;
         a.q_raw = g->qp;
         a.prepared = 1;
     }
-    e = launch_attention(a, g->stream);
+    e = g->window ? enqueue_attend(g, layer, a, true) : launch_attention(a, g->stream);
     if (e != hipSuccess) return e;
-    if (attention_oproj_fits(a, d.o)) {
+    if (!g->window && attention_oproj_fits(a, d.o)) {
         const int np = g->nh / ATTN_OPROJ_HEADS;
         e = launch_attention_oproj(a, d.o, g->parts, g->stream);
         return e == hipSuccess ? launch_attn_fold(g->x, g->parts, np, g->H, g->stream, n) : e;
     }
-    e = launch_attention_merge(a, g->stream);
+    if (!g->window) e = launch_attention_merge(a, g->stream);
     if (e != hipSuccess) return e;
     gemv_args go;
     memset(&go, 0, sizeof(go));
@@ -2399,6 +2486,21 @@ static bool set_rows(vitna_cuda_model* g, const vitna_cuda_row_t* rows, size_t n
     g->rows_n = (int)n;
     g->rows_one_seq = true;
     for (size_t i = 1; i < n; i++) g->rows_one_seq &= rows[i].seq == rows[0].seq;
+    g->rows_prefix = g->rows_own = 0;
+    for (size_t i = 0; g->sharing && i < n; i++) unshare(g, rows[i].seq, rows[i].pos);
+    if (g->sharing && !g->rows_one_seq) { /* (a prompt's chunk reads its one sequence) */
+        int prefix = 0, own = 1;
+        for (size_t i = 0; i < n; i++) {
+            const seq_share x = g->share[rows[i].seq];
+            if (i && x.len && x.len == g->share[rows[i - 1].seq].len && x.base == g->share[rows[i - 1].seq].base) prefix = std::max(prefix, (int)x.len);
+            own = std::max(own, (int)rows[i].pos + 1 - x.len);
+        }
+        if (prefix) {
+            for (g->rows_prefix = 64; g->rows_prefix < prefix;) g->rows_prefix <<= 1;
+            for (g->rows_own = 64; g->rows_own < own;) g->rows_own <<= 1;
+            if (!push_share(g, err, err_len)) return false;
+        }
+    }
     g->pass_exact = false; /* vitna_cuda_moe_rows_route decides at layer 0 */
     g->parts_n = 0; /* a pass of rows owns x's rows: no one row's attention parts are pending any more */
     g->rows_shared_seq = shared;
@@ -2656,7 +2758,8 @@ static bool ensure_rows_graph(vitna_cuda_model* g, int n, int head, char* err, s
     int pick = 0;
     for (int i = 0; i < ROWS_GRAPHS; i++) {
         const auto& r = g->rg[i];
-        if (r.n == n && r.shared == g->rows_shared_seq && r.one_seq == g->rows_one_seq && r.fast == fast && r.splits == g->splits_grid && r.head == head) {
+        if (r.n == n && r.shared == g->rows_shared_seq && r.one_seq == g->rows_one_seq && r.fast == fast && r.splits == g->splits_grid && r.head == head &&
+            r.prefix == g->rows_prefix && r.own == g->rows_own) {
             g->rg[i].used = ++g->rg_clock;
             g->rg_cur = i;
             return true;
@@ -2685,6 +2788,8 @@ static bool ensure_rows_graph(vitna_cuda_model* g, int n, int head, char* err, s
     r.shared = g->rows_shared_seq;
     r.one_seq = g->rows_one_seq;
     r.splits = g->splits_grid;
+    r.prefix = g->rows_prefix;
+    r.own = g->rows_own;
     r.head = head;
     r.used = ++g->rg_clock;
     g->rg_cur = pick;
@@ -2725,5 +2830,258 @@ extern "C" bool vitna_hip_time_rows(struct vitna_cuda_model* g, const vitna_cuda
     float ms = 0;
     HIP_TRY(hipEventElapsedTime(&ms, ev.t0, ev.t1), "events");
     *ms_per_step = (double)ms / steps;
+    return true;
+}
+
+/* ---- several continuations at once (include/vitna_serve.h) ---- */
+
+/* Positions from on of sequence seq change: what it shared there with others it shares no more, nor they with it. */
+static void unshare(vitna_cuda_model* g, int seq, int from) {
+    if (g->held[seq] <= from) return;
+    g->held[seq] = from;
+    bool some = false;
+    for (int s = 0; s < g->seqs; s++) {
+        seq_share& x = g->share[s];
+        if ((s == seq || x.base == seq) && x.len > from) x.len = from;
+        some |= x.len != 0;
+    }
+    g->sharing = some;
+}
+
+/* Everything the calls below use, made once. The attention's scratch holds any pass (the graphs keep its address): up to
+   EXACT_ROWS rows of attend_splits parts, up to ROWS_MAX rows cut as launch_attend cuts them. */
+static bool ensure_serve(vitna_cuda_model* g, char* err, size_t err_len) {
+    if (!g || g->lost) return fail(err, err_len, "the device model is not usable");
+    if (!g->attention) return fail(err, err_len, "this model has no attention");
+    HIP_TRY(hipSetDevice(g->device), "selecting the model's device");
+    if (!g->attend_buf) {
+        size_t most = 0;
+        attend_args t = model_attend(g, 0, 1);
+        t.window = 0;
+        t.own_max = t.shared_max = g->ctx;
+        for (t.n = 1; t.n <= ROWS_MAX; t.n++)
+            for (int kind = 0; kind < 4; kind++) {
+                attend_args x = t;
+                if (kind == 1) x.shared_max = 0;
+                if (kind == 2) { x.shared_max = 0; x.run = 1; }
+                if (kind == 3) { x.shared_max = 0; x.splits = 64; }
+                if (kind == 3 && x.n > EXACT_ROWS) continue;
+                most = std::max(most, attend_work(x));
+            }
+        if (!dalloc(g, &g->attend_buf, most, "the attention's scratch", err, err_len)) return false;
+        g->attend_bytes = most;
+    }
+    if (!g->serve_copied) HIP_TRY(hipEventCreateWithFlags(&g->serve_copied, hipEventDisableTiming), "an event");
+    if (!g->share_dev && !dalloc(g, &g->share_dev, (size_t)g->seqs * sizeof(int2), "the sequences' table", err, err_len)) return false;
+    if (!g->share_host) HIP_TRY(hipHostMalloc((void**)&g->share_host, (size_t)g->seqs * sizeof(seq_share), 0), "page-locked memory");
+    if (!g->fork_dev && !dalloc(g, &g->fork_dev, 4 * ROWS_MAX * 4, "a reordering's table", err, err_len)) return false;
+    if (!g->fork_host) HIP_TRY(hipHostMalloc((void**)&g->fork_host, 4 * ROWS_MAX * 4, 0), "page-locked memory");
+    if (!g->beam_dev && !dalloc(g, &g->beam_dev, ROWS_MAX * 20, "a beam step's results", err, err_len)) return false;
+    if (!g->beam_host) HIP_TRY(hipHostMalloc((void**)&g->beam_host, ROWS_MAX * 20, 0), "page-locked memory");
+    try {
+        if (g->share.empty()) {
+            g->held.assign(g->seqs, 0);
+            g->share.assign(g->seqs, seq_share{0, 0});
+        }
+    } catch (const std::bad_alloc&) {
+        return fail(err, err_len, "no memory for a table of %d sequences", g->seqs);
+    }
+    return true;
+}
+
+static bool push_share(vitna_cuda_model* g, char* err, size_t err_len) {
+    HIP_TRY(hipEventSynchronize(g->serve_copied), "waiting for the previous copies");
+    memcpy(g->share_host, g->share.data(), (size_t)g->seqs * sizeof(seq_share));
+    HIP_TRY(hipMemcpyAsync(g->share_dev, g->share_host, (size_t)g->seqs * sizeof(seq_share), hipMemcpyHostToDevice, g->stream), "copying the sequences' table");
+    HIP_TRY(hipEventRecord(g->serve_copied, g->stream), "recording the copies");
+    return true;
+}
+
+/* A reordering of groups x width sequences (list), each from its parents[i] of its group, positions spans; enqueued. */
+static bool move_caches(vitna_cuda_model* g, const int32_t* list, const int32_t* parents, const int32_t* spans, int groups, int width, int longest,
+                        char* err, size_t err_len) {
+    const size_t n = (size_t)groups * width;
+    HIP_TRY(hipEventSynchronize(g->serve_copied), "waiting for the previous copies");
+    memcpy(g->fork_host, list, n * 4);
+    memcpy(g->fork_host + ROWS_MAX, parents, n * 4);
+    memcpy(g->fork_host + 2 * ROWS_MAX, spans, (size_t)groups * 8);
+    HIP_TRY(hipMemcpyAsync(g->fork_dev, g->fork_host, (2 * ROWS_MAX + 2 * (size_t)groups) * 4, hipMemcpyHostToDevice, g->stream), "copying the reordering");
+    HIP_TRY(hipEventRecord(g->serve_copied, g->stream), "recording the copies");
+    kv_reorder_args a = {};
+    a.k = reinterpret_cast<char*>(g->k_cache); a.v = reinterpret_cast<char*>(g->v_cache);
+    a.layer_bytes = g->layer_kv * 4; a.seq_bytes = a.layer_bytes * g->NL; a.pos_bytes = (size_t)g->nkv * g->hd * 4; a.head_bytes = a.dim_bytes = (size_t)g->hd * 4;
+    a.n_kv = g->nkv; a.ctx = g->ctx; a.seqs = g->seqs; a.layers = g->NL;
+    a.list = g->fork_dev; a.parents = g->fork_dev + ROWS_MAX; a.spans = g->fork_dev + 2 * ROWS_MAX;
+    a.groups = groups; a.width = width; a.longest = longest;
+    return check_launch(g, launch_kv_reorder(a, g->stream), "copying caches", err, err_len);
+}
+
+extern "C" bool vitna_hip_set_window(struct vitna_cuda_model* g, size_t window, size_t sinks, char* err, size_t err_len) {
+    if (!ensure_serve(g, err, err_len)) return false;
+    const int w = window >= (size_t)g->ctx ? 0 : (int)window, k = w ? (int)std::min(sinks, (size_t)g->ctx) : 0;
+    if (w == g->window && k == g->sinks) return true;
+    HIP_TRY(hipStreamSynchronize(g->stream), "waiting for the device");
+    if (g->graph_ready) {
+        (void)hipGraphExecDestroy(g->step_graph);
+        (void)hipGraphDestroy(g->step_graph_src);
+        g->graph_ready = false;
+    }
+    drop_rows_graphs(g);
+    g->window = w;
+    g->sinks = k;
+    return true;
+}
+
+extern "C" bool vitna_hip_kv_fork(struct vitna_cuda_model* g, size_t src, size_t n_pos, const int32_t* dst, size_t n, char* err, size_t err_len) {
+    if (!ensure_serve(g, err, err_len)) return false;
+    if (src >= (size_t)g->seqs) return fail(err, err_len, "sequence %zu: the cache holds %d", src, g->seqs);
+    if (n_pos > (size_t)g->ctx) return fail(err, err_len, "%zu positions: the cache holds %d", n_pos, g->ctx);
+    if (n > ROWS_MAX || (n && !dst)) return fail(err, err_len, "%zu sequences to fork into; at most %d", n, ROWS_MAX);
+    int32_t all[ROWS_MAX];
+    std::copy(dst, dst + n, all);
+    std::sort(all, all + n);
+    for (size_t i = 0; i < n; i++) {
+        if (all[i] < 0 || all[i] >= g->seqs) return fail(err, err_len, "sequence %d: the cache holds %d", all[i], g->seqs);
+        if ((size_t)all[i] == src || (i && all[i] == all[i - 1])) return fail(err, err_len, "sequence %d is forked into itself or twice", all[i]);
+    }
+    if (!n || !n_pos) return true;
+    /* the sequence whose positions they all are: src's own base, if it shares that many with it */
+    const seq_share has = g->share[src];
+    const int base = has.len >= (int)n_pos ? has.base : (int)src;
+    const int32_t span[2] = {0, (int32_t)n_pos};
+    for (size_t at = 0; at < n; at += VITNA_HIP_BEAMS_MAX - 1) {
+        const int many = (int)std::min<size_t>(n - at, VITNA_HIP_BEAMS_MAX - 1);
+        int32_t list[VITNA_HIP_BEAMS_MAX], parents[VITNA_HIP_BEAMS_MAX] = {};
+        list[0] = (int32_t)src;
+        for (int i = 0; i < many; i++) {
+            list[1 + i] = dst[at + i];
+            unshare(g, dst[at + i], 0);
+        }
+        if (!move_caches(g, list, parents, span, 1, many + 1, (int)n_pos, err, err_len)) return false;
+    }
+    for (size_t i = 0; i < n; i++) {
+        g->share[dst[i]] = seq_share{base, (int32_t)n_pos};
+        g->held[dst[i]] = (int32_t)n_pos;
+    }
+    if (base == (int)src) g->share[src] = seq_share{base, (int32_t)n_pos};
+    g->held[src] = std::max(g->held[src], (int32_t)n_pos);
+    g->held[base] = std::max(g->held[base], (int32_t)n_pos);
+    g->sharing = true;
+    return true;
+}
+
+extern "C" bool vitna_hip_beam_step(struct vitna_cuda_model* g, vitna_cuda_row_t* rows, size_t groups, size_t width, float* scores,
+                                    uint8_t* ended, int32_t end_token, int32_t* parents, char* err, size_t err_len) {
+    if (!ensure_serve(g, err, err_len)) return false;
+    if (!experts_resident(g, err, err_len)) return false;
+    if (!rows || !scores || !ended) return fail(err, err_len, "rows, scores and ended are needed");
+    if (width < 1 || width > VITNA_HIP_BEAMS_MAX) return fail(err, err_len, "%zu beams; 1 to %d are served", width, VITNA_HIP_BEAMS_MAX);
+    if (groups < 1 || groups > ROWS_MAX / width) return fail(err, err_len, "%zu groups of %zu beams: at most %d rows a pass", groups, width, ROWS_MAX);
+    const size_t n = groups * width;
+    if (end_token >= g->V) return fail(err, err_len, "token %d is outside the vocabulary of %d", end_token, g->V);
+    for (size_t i = 0; i < n; i++) {
+        if (end_token < 0 && ended[i]) return fail(err, err_len, "beam %zu has ended, and there is no end token", i);
+        for (size_t j = 0; j < i; j++)
+            if (rows[j].seq == rows[i].seq) return fail(err, err_len, "beams %zu and %zu are both in sequence %d", j, i, rows[i].seq);
+    }
+    const size_t need = beam_select_work((int)groups, (int)width, (size_t)g->V, (int)width);
+    if (need > g->beam_work_bytes) {
+        if (!dalloc(g, &g->beam_work, need, "the selection's scratch", err, err_len)) return false;
+        g->beam_work_bytes = need;
+    }
+    if (!set_rows(g, rows, n, err, err_len)) return false;
+    if (!ensure_rows_graph(g, (int)n, HEAD_ALL, err, err_len)) return false;
+    HIP_TRY(hipGraphLaunch(g->rg[g->rg_cur].exec, g->stream), "launching the rows step");
+    g->last_step_mega = false;
+    /* [scores | best | parents | tokens | ended], ROWS_MAX of each */
+    HIP_TRY(hipEventSynchronize(g->serve_copied), "waiting for the previous copies");
+    float *d_scores = reinterpret_cast<float*>(g->beam_dev), *h_scores = reinterpret_cast<float*>(g->beam_host);
+    float *d_best = d_scores + ROWS_MAX, *h_best = h_scores + ROWS_MAX;
+    int32_t *d_parents = reinterpret_cast<int32_t*>(d_best + ROWS_MAX), *h_parents = reinterpret_cast<int32_t*>(h_best + ROWS_MAX);
+    int32_t *d_tokens = d_parents + ROWS_MAX, *h_tokens = h_parents + ROWS_MAX;
+    uint8_t *d_ended = reinterpret_cast<uint8_t*>(d_tokens + ROWS_MAX), *h_ended = reinterpret_cast<uint8_t*>(h_tokens + ROWS_MAX);
+    memcpy(h_scores, scores, n * 4);
+    memcpy(h_ended, ended, n);
+    HIP_TRY(hipMemcpyAsync(d_scores, h_scores, n * 4, hipMemcpyHostToDevice, g->stream), "copying the scores");
+    HIP_TRY(hipMemcpyAsync(d_ended, h_ended, n, hipMemcpyHostToDevice, g->stream), "copying what has ended");
+    beam_select_args a = {};
+    a.logits = g->vocab; a.stride = a.vocab = (size_t)g->V;
+    a.groups = (int)groups; a.width = a.keep = (int)width;
+    a.scores = d_scores; a.ended = end_token < 0 ? nullptr : d_ended; a.end_token = end_token;
+    a.best = d_best; a.parents = d_parents; a.tokens = d_tokens; a.work = g->beam_work;
+    if (!check_launch(g, launch_beam_select(a, g->stream), "the selection", err, err_len)) return false;
+    HIP_TRY(hipMemcpyAsync(h_best, d_best, 3 * ROWS_MAX * 4, hipMemcpyDeviceToHost, g->stream), "copying the selection");
+    HIP_TRY(hipEventRecord(g->serve_copied, g->stream), "recording the copies");
+    HIP_TRY(hipStreamSynchronize(g->stream), "running the beam step");
+
+    /* The first continuation of a beam stays in its sequence; the others take those of beams that end, and copy. */
+    int32_t list[ROWS_MAX], from[ROWS_MAX], spans[2 * ROWS_MAX];
+    vitna_cuda_row_t next[ROWS_MAX];
+    uint8_t done[ROWS_MAX];
+    int longest = 0;
+    bool moves = false;
+    for (size_t q = 0; q < groups; q++) {
+        const size_t at = q * width;
+        int slot[VITNA_HIP_BEAMS_MAX];                   /* of a continuation */
+        bool taken[VITNA_HIP_BEAMS_MAX] = {};            /* a beam's sequence */
+        for (size_t j = 0; j < width; j++) {
+            const int p = h_parents[at + j];
+            slot[j] = -1;
+            if (p >= 0 && !taken[p]) {
+                slot[j] = p;
+                taken[p] = true;
+            }
+        }
+        int free_ = 0, to = 0, common = g->ctx, base = -1;
+        for (size_t j = 0; j < width; j++) {
+            list[at + j] = rows[at + j].seq;
+            from[at + j] = (int32_t)j;
+        }
+        for (size_t j = 0; j < width; j++) {
+            const int p = h_parents[at + j];
+            if (slot[j] < 0) {
+                while (taken[free_]) free_++;
+                slot[j] = free_;
+                taken[free_] = true;
+                if (p >= 0) {
+                    from[at + free_] = p;
+                    moves = true;
+                    to = std::max(to, rows[at + p].pos + 1);
+                }
+            }
+            vitna_cuda_row_t& r = next[at + j];
+            if (p < 0) { /* no continuation is left for it */
+                r = rows[at + slot[j]];
+                done[at + j] = ended[at + slot[j]];
+            } else {
+                const bool over = ended[at + p] != 0; /* an ended beam keeps its place */
+                r = vitna_cuda_row_t{h_tokens[at + j], rows[at + p].pos + (over ? 0 : 1), rows[at + slot[j]].seq};
+                done[at + j] = over || (end_token >= 0 && h_tokens[at + j] == end_token);
+                if (over) r.token = rows[at + p].token;
+            }
+        }
+        /* what the group's sequences share stays where it is */
+        for (size_t j = 0; j < width; j++) {
+            const seq_share x = g->share[list[at + j]];
+            if (!j) base = x.base;
+            common = x.base == base ? std::min(common, (int)x.len) : 0;
+        }
+        spans[2 * q] = common;
+        spans[2 * q + 1] = to;
+        longest = std::max(longest, to - common);
+    }
+    if (moves) {
+        if (g->sharing)
+            for (size_t q = 0; q < groups; q++)
+                for (size_t j = 0; j < width; j++)
+                    if (from[q * width + j] != (int32_t)j) unshare(g, list[q * width + j], spans[2 * q]);
+        if (longest > 0 && !move_caches(g, list, from, spans, (int)groups, (int)width, longest, err, err_len)) return false;
+    }
+    for (size_t i = 0; i < n; i++) {
+        rows[i] = next[i];
+        ended[i] = done[i];
+        scores[i] = h_best[i];
+        if (parents) parents[i] = h_parents[i];
+    }
     return true;
 }

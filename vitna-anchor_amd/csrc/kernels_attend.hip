@@ -53,7 +53,18 @@ struct attend_parts {
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ attend_row row_of(const attend_args& a, int r) {
-    attend_row x = a.rows ? a.rows[r] : attend_row{a.run_seq, a.run_pos + r, 0, 0};
+    attend_row x = {a.run_seq, a.run_pos + r, 0, 0};
+    if (a.rows) {
+        x = a.rows[r];
+    } else if (a.recs) {
+        x.seq = a.recs[r].seq;
+        x.pos = a.recs[r].pos;
+        if (a.share && x.seq >= 0 && x.seq < a.seqs) {
+            const int2 s = a.share[x.seq];
+            x.base = s.x;
+            x.shared = s.y;
+        }
+    }
     if (a.run) x.shared = 0;
     const bool ok = x.seq >= 0 && x.seq < a.seqs && x.pos >= 0 && x.pos < a.ctx && x.shared >= 0 && (!x.shared || (x.base >= 0 && x.base < a.seqs));
     if (!ok) x = attend_row{0, -1, 0, 0};
@@ -341,7 +352,7 @@ struct group_span {
 template <bool RUN>
 __device__ __forceinline__ group_span group_seen(const attend_args& a, const attend_row* srow, int first, int next) {
     group_span s;
-    s.seq = __builtin_amdgcn_readfirstlane(RUN ? (a.rows ? srow[first].seq : a.run_seq) : srow[first].base);
+    s.seq = __builtin_amdgcn_readfirstlane(RUN ? (a.recs ? srow[first].seq : a.run_seq) : srow[first].base);
     int end = __builtin_amdgcn_readfirstlane(srow[first].shared), least = 0;
     if (RUN || a.window) {
         /* the rows' furthest and nearest positions */
@@ -968,7 +979,8 @@ static attend_parts plan(const attend_args& a) {
         const bool few = a.n * G <= FEW_COLUMNS;
         p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), std::max<long>(1, (few ? 2 : 1) * blocks / ((long)p.tiles * a.n_kv)));
     }
-    p.own = (int)std::min<long>(std::min<long>((seen + 16 * OWN_WAVES - 1) / (16 * OWN_WAVES), 256), std::max<long>(1, 1024 / ((long)a.n * a.n_kv)));
+    p.own = (int)std::min<long>(std::min<long>((seen + 16 * OWN_WAVES - 1) / (16 * OWN_WAVES), ATTEND_SPLITS_MAX), std::max<long>(1, 1024 / ((long)a.n * a.n_kv)));
+    if (a.splits) p.own = std::min(a.splits, ATTEND_SPLITS_MAX);
     return p;
 }
 

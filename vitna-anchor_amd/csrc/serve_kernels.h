@@ -9,7 +9,7 @@
 #ifndef SERVE_KERNELS_H
 #define SERVE_KERNELS_H
 
-#include "vitna_hip_internal.h"
+#include "vitna_kernels.h"
 
 /* Maximum over the wave of unsigned numbers, in every lane. */
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
@@ -38,17 +38,22 @@ struct attend_args {
     float* out;
     size_t out_stride;
     int n;
-    /* the rows: n of them in rows, or (rows null) positions run_pos .. run_pos + n - 1 of sequence run_seq */
+    /* the rows: n of them in rows; or a model's in recs, which share what share (of each sequence: base and number of
+       positions; null: nothing) says; or, both null, positions run_pos .. run_pos + n - 1 of sequence run_seq */
     const attend_row* rows;
+    const row_rec* recs;
+    const int2* share;
     int run_seq, run_pos;
-    /* 1: the rows are tokens of one sequence (a prompt's chunk), rows[i].seq the same for all and nothing shared */
+    /* 1: the rows are tokens of one sequence (a prompt's chunk) and share nothing */
     int run;
     int own_max, shared_max; /* the longest own part and the longest shared prefix, about: they size the launch */
+    int splits;              /* 0, or the blocks that a row's own part is split over whatever n is (then its bits are, too) */
     void* work;
     size_t work_bytes;
 };
 /* Bytes of work that launch_attend needs for a's shapes (its pointers are not read). */
 size_t attend_work(const attend_args& a);
+#define ATTEND_SPLITS_MAX 256 /* of a row's own part */
 hipError_t launch_attend(const attend_args& a, hipStream_t s);
 
 struct beam_select_args {

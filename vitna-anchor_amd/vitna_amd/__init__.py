@@ -394,6 +394,10 @@ def _hip():
         "vitna_hip_beam_select_work": (C.c_size_t, [C.c_size_t] * 4),
         "vitna_hip_beam_select": (C.c_bool, [P, *[C.c_size_t] * 5, P, P, C.c_int32, P, P, P, P, C.c_size_t, P, *E]),
         "vitna_hip_kv_reorder": (C.c_bool, [C.POINTER(KvView), C.c_size_t, C.c_size_t, P, P, P, C.c_size_t, C.c_size_t, C.c_size_t, P, *E]),
+        "vitna_hip_set_window": (C.c_bool, [P, C.c_size_t, C.c_size_t, *E]),
+        "vitna_hip_kv_fork": (C.c_bool, [P, C.c_size_t, C.c_size_t, C.POINTER(C.c_int32), C.c_size_t, *E]),
+        "vitna_hip_beam_step": (C.c_bool, [P, C.POINTER(RowT), C.c_size_t, C.c_size_t, _FP, C.POINTER(C.c_uint8), C.c_int32,
+                                           C.POINTER(C.c_int32), *E]),
         "vitna_hip_time_ffn": (C.c_bool, [P, C.c_int, C.POINTER(C.c_double), *E]),
         "vitna_hip_time_kernel": (C.c_bool, [P, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double),
                                              C.POINTER(C.c_double), *E]),
@@ -548,6 +552,56 @@ class Device:
         ptrs = self._row_pointers(out, only) if logits else None
         self._ok(self.lib.vitna_hip_moe_rows_step(self.g, self._rows(rows), n, ptrs, self.err, 512))
         return out
+
+    # --- several continuations at once (include/vitna_serve.h) ---
+    def set_window(self, window, sinks=0):
+        """Later steps and passes attend to a row's last window positions and its sequence's first sinks (0: to all)."""
+        self._ok(self.lib.vitna_hip_set_window(self.g, window, sinks, self.err, 512))
+
+    def kv_fork(self, src, n_pos, dst):
+        """The first n_pos positions of sequence src into the sequences dst, which share them with it from then on."""
+        d = np.ascontiguousarray(dst, np.int32)
+        self._ok(self.lib.vitna_hip_kv_fork(self.g, src, n_pos, _i32(d), d.size, self.err, 512))
+
+    def beam_step(self, rows, width, scores, ended, end_token=-1):
+        """One step of beam search for len(rows) / width prompts: (rows, scores, ended, parents) of the continuations."""
+        n = len(rows)
+        if width < 1 or n % width:
+            raise ValueError("%d rows are no groups of %d beams" % (n, width))
+        r = self._rows(rows)
+        s = np.array(scores, np.float32)
+        e = np.array(ended, np.uint8)
+        p = np.empty(n, np.int32)
+        if s.shape != (n,) or e.shape != (n,):
+            raise ValueError("a score and an ended flag for each of %d rows" % n)
+        self._ok(self.lib.vitna_hip_beam_step(self.g, r, n // width, width, fptr(s), e.ctypes.data_as(C.POINTER(C.c_uint8)), end_token,
+                                              _i32(p), self.err, 512))
+        return [(x.token, x.pos, x.seq) for x in r], s, e, p
+
+    def beam_search(self, prompt, width, steps, end_token=-1, seqs=None):
+        """The width best continuations of prompt (a list of tokens) by at most steps tokens, in sequences seqs (by default
+        0 .. width - 1): [(tokens, sum of log probabilities)], best first. A continuation ends with end_token."""
+        if not len(prompt) or steps < 1 or width < 1:
+            raise ValueError("a token, a step and a beam at least")
+        seqs = list(range(width)) if seqs is None else list(seqs)
+        if len(seqs) != width:
+            raise ValueError("%d sequences for %d beams" % (len(seqs), width))
+        before = len(prompt) - 1
+        for at in range(0, before, self.rows_max()):
+            chunk = prompt[at:min(at + self.rows_max(), before)]
+            self.rows_step([(int(t), at + i, seqs[0]) for i, t in enumerate(chunk)], logits=False)
+        self.kv_fork(seqs[0], before, seqs[1:])
+        rows = [(int(prompt[-1]), before, s) for s in seqs]
+        scores, ended = np.full(width, -np.inf, np.float32), np.zeros(width, np.uint8)
+        scores[0] = 0.0
+        texts = [[] for _ in seqs]
+        for _ in range(steps):
+            was = ended
+            rows, scores, ended, parents = self.beam_step(rows, width, scores, ended, end_token)
+            texts = [[] if p < 0 else texts[p] + ([] if was[p] else [rows[i][0]]) for i, p in enumerate(parents)]
+            if np.all((ended != 0) | (scores == -np.inf)):
+                break
+        return [(t, float(s)) for t, s in zip(texts, scores) if s > -np.inf]
 
     def step_async(self, seq, token, pos):
         self._ok(self.lib.vitna_hip_moe_step_async(self.g, seq, token, pos, self.err, 512))
