@@ -48,6 +48,10 @@ struct attend_parts {
     float* acc;  /* [n][n_kv][splits][G][hd]: its weighted values; unset where the sum is 0 */
     int own, tile; /* splits of the own parts and of the tiles' */
     int tiles;     /* tiles of rows */
+    /* a run's chunks ready for LDS (attend_image_kernel): slots of them for each key-value head; 0: none */
+    int slots;
+    char* images;  /* [n_kv][slots] */
+    int4* meta;    /* [0]: where the slots lie; [1 + n_kv slots]: of each, its keys' and values' powers of two, and the positions whose values are no numbers */
 };
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -457,61 +461,161 @@ struct tile_shape {
     static_assert(U >= 1 && U * NT == 16 * CC, "whole groups a thread");
 };
 
-/* Split split of what the columns of rows row0 + 0 .. n_rows - 1 see together: RUN, rows of one sequence, each up to itself;
-   otherwise a group's shared prefix. srow are the rows. */
-template <int HD, typename T, int NW, bool RUN>
-__device__ __forceinline__ void group_part(const attend_args& a, const attend_parts& p, int split, int h, int row0, int n_rows,
-                                           const attend_row* srow, const group_span& s_, char* lds) {
-    typedef tile_shape<HD, T, NW> sh;
-    constexpr bool PARTS = sh::PARTS, SCALED = sh::SCALED;
-    constexpr int KS = HD / 16, DT = HD / 32, U = sh::U, CC = sh::CC, HALF = sh::HALF;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c32 = lane & 31, hh = lane >> 5;
-    const int G = a.n_heads / a.n_kv, S = p.own + p.tile;
-    /* Keys [part][64 positions][HD] in pieces of 8 dimensions, piece x of position t at x ^ t mod (HD / 8). Values
-       [part][HD][64 positions] in units of two pieces of 4 positions, those of one MFMA operand (positions 16 s + 4 hh ..
-       and 16 s + 8 + 4 hh ..: unit 2 s + hh), unit x of dimension d at x ^ (d / 2 ^ d / 16) mod 8. Sixteen lanes'
-       16-byte reads then take every bank once, and all places are one lane's ^ and + a constant. */
-    uint32_t* smax = reinterpret_cast<uint32_t*>(lds); /* [2][NW]: magnitudes of keys, of values */
-    uint32_t* sbad = smax + 2 * NW;                    /* positions whose values are not finite */
-    char* sk = lds + sh::HEAD;
-    char* sv = sk + (PARTS ? 2 : 1) * HALF * 2;
-    auto key_to = [&](int pg, int cc) { return (uint32_t)(4 * pg * HD * 2 + (((cc >> 1) ^ ((4 * pg) & (HD / 8 - 1))) << 4) + 8 * (cc & 1)); };
-    auto value_to = [&](int pg, int cc) {
-        const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1;
-        return (uint32_t)(4 * cc * 128 + ((unit ^ (((2 * cc) ^ (cc >> 2)) & 7)) << 4) + 8 * half);
-    };
+/* Places in a chunk's LDS (and image). Keys [part][64 positions][HD] in pieces of 8 dimensions, piece x of position t at
+   x ^ t mod (HD / 8). Values [part][HD][64 positions] in units of two pieces of 4 positions, those of one MFMA operand
+   (positions 16 s + 4 hh .. and 16 s + 8 + 4 hh ..: unit 2 s + hh), unit x of dimension d at x ^ (d / 2 ^ d / 16) mod 8.
+   Sixteen lanes' 16-byte reads then take every bank once, and all places are one lane's ^ and + a constant. Thread group
+   (pg, cc) holds positions 4 pg + i and dimensions 4 cc + d: key i at (key_to ^ i << 4) + i rows, values d at
+   (value_to ^ (d / 2) << 4) + d rows. */
+template <int HD>
+__device__ __forceinline__ uint32_t key_to(int pg, int cc) {
+    return (uint32_t)(4 * pg * HD * 2 + (((cc >> 1) ^ ((4 * pg) & (HD / 8 - 1))) << 4) + 8 * (cc & 1));
+}
+__device__ __forceinline__ uint32_t value_to(int pg, int cc) {
+    const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1;
+    return (uint32_t)(4 * cc * 128 + ((unit ^ (((2 * cc) ^ (cc >> 2)) & 7)) << 4) + 8 * half);
+}
 
-    /* seen, in chunks of 64 */
-    const int seq = s_.seq, sink = s_.sink, from = s_.from, end = s_.end;
-    const int n_sink = (sink + 63) >> 6, n_chunks = n_sink + ((end - from + 63) >> 6);
-    const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
-    /* the lane's column */
-    const int col = 32 * wave + c32, lr = col / G, g = col - lr * G;
-    const bool there = lr < n_rows;
-    const attend_row me = srow[there ? lr : 0];
-    const int last = !there ? -1 : RUN ? me.pos : min(me.shared, me.pos + 1) - 1; /* the last position it may see here */
-    const int low = a.window ? me.pos - a.window + 1 : INT32_MIN;
-    const size_t row = (size_t)(row0 + lr), part = ((row * a.n_kv + h) * S + p.own + split) * G + g;
-    if (c0 >= c1) {
-        if (!there || hh) return;
-        if (S > 1) p.ml[part] = make_float2(-INFINITY, 0.0f);
-        else
-            for (int i = 0; i < HD / 4; i++) reinterpret_cast<float4*>(a.out + row * a.out_stride + (size_t)(h * G + g) * HD)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        return;
+/* A thread's share of 64 positions' keys or values: U groups of 4 positions x 4 dimensions. */
+template <int HD, typename T, int NT>
+struct chunk_share {
+    static constexpr int CC = HD / 4, U = 16 * CC / NT;
+    vec<T, 4> x[U][4];
+    /* positions t0 .. t1 - 1 (64 at most) of src (a head's positions); those behind t1 read the last again: their scores are masked */
+    __device__ __forceinline__ void fetch(const T* src, size_t pos_stride, int t0, int t1) {
+        const uint32_t most = (uint32_t)(min(t1 - t0, 64) - 1), pos_bytes = (uint32_t)(pos_stride * sizeof(T)); /* 64 of them stay within 31 bits */
+        const char* from = reinterpret_cast<const char*>(src + (size_t)t0 * pos_stride);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = threadIdx.x + NT * u, pg = at / CC, cc = at % CC;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                x[u][i] = *reinterpret_cast<const vec<T, 4>*>(from + (min((uint32_t)(4 * pg + i), most) * pos_bytes + (uint32_t)(4 * sizeof(T)) * cc));
+        }
     }
-    if (tid < 2) sbad[tid] = 0;
+    /* the wave's largest magnitude to its slot; finite: of the numbers among them */
+    __device__ __forceinline__ void publish(uint32_t* slots, bool finite = false) const {
+        uint32_t mag = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    uint32_t v = magnitude((float)x[u][i][d]);
+                    if (finite && v >= MAG_INF) v = 0;
+                    mag = max(mag, v);
+                }
+        mag = wave_umax(mag);
+        if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = mag;
+    }
+    static __device__ __forceinline__ uint32_t largest(const uint32_t* slots) {
+        uint32_t mag = slots[0];
+#pragma unroll
+        for (int w = 1; w < NT / 64; w++) mag = max(mag, slots[w]);
+        return (uint32_t)__builtin_amdgcn_readfirstlane((int)mag);
+    }
+    /* the finite ones' largest, where some are not: a rare way round, of the whole block */
+    __device__ __forceinline__ uint32_t finite_largest(uint32_t* slots) const {
+        lds_barrier(); /* every wave has read the slots */
+        publish(slots, true);
+        lds_barrier();
+        return largest(slots);
+    }
+    /* values that are no numbers taken out (a weight of 0 would make NaN of them), their positions' bits set in bad */
+    __device__ __forceinline__ void take_out(uint32_t* bad) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int pg = (threadIdx.x + NT * u) / CC;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                bool b = false;
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    if (magnitude((float)x[u][i][d]) >= MAG_INF) {
+                        x[u][i][d] = (T)0.0f;
+                        b = true;
+                    }
+                if (b) atomicOr(&bad[(4 * pg + i) >> 5], 1u << ((4 * pg + i) & 31));
+            }
+        }
+    }
+    __device__ __forceinline__ void store_keys(char* sk, float f) const {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = threadIdx.x + NT * u, pg = at / CC, cc = at % CC;
+#pragma unroll
+            for (int i = 0; i < 4; i++) put(sk + (key_to<HD>(pg, cc) ^ (i << 4)) + i * HD * 2, x[u][i][0], x[u][i][1], x[u][i][2], x[u][i][3], f);
+        }
+    }
+    __device__ __forceinline__ void store_values(char* sv, float f) const {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = threadIdx.x + NT * u, pg = at / CC, cc = at % CC;
+#pragma unroll
+            for (int d = 0; d < 4; d++) put(sv + (value_to(pg, cc) ^ ((d >> 1) << 4)) + d * 128, x[u][0][d], x[u][1][d], x[u][2][d], x[u][3][d], f);
+        }
+    }
+    static __device__ __forceinline__ void put(char* to, T a, T b, T c, T d, float f) {
+        uint2 hi, lo;
+        if constexpr (std::is_same<T, _Float16>::value) hi = __builtin_bit_cast(uint2, vec<T, 4>{a, b, c, d});
+        else cut4((float)a, (float)b, (float)c, (float)d, f, hi, lo);
+        *reinterpret_cast<uint2*>(to) = hi;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(to + 64 * HD * 2) = lo;
+    }
+};
+
+/* A wave's 32 columns: queries, running maximum, sum and weighted values. Column 32 wave + c32 is row row0 + x / G, query
+   head h G + x mod G; lanes c32 and c32 + 32 hold its halves. */
+template <int HD, typename T>
+struct wave_columns {
+    static constexpr bool PARTS = sizeof(T) == 4, SCALED = !std::is_same<T, _Float16>::value;
+    static constexpr int KS = HD / 16, DT = HD / 32, LO = 64 * HD * 2; /* bytes from a hi part to its lo part */
     h8v qh[KS], ql[KS];
-    float to_score; /* from the products' sums to scores in units of log 2, with the keys' power of two */
-    {
-        /* The wave's 32 columns through 4 KB of LDS of its own, 32 dimensions at a time: loaded 128 bytes a column (a lane
-           a column would ask for 64 lines an instruction, 18000 cycles a block), taken as operand 16 s + 8 hh .. */
+    f16v S[2], O[DT];
+    float to_score; /* from the products' sums to scores in units of log 2, but for the keys' power of two */
+    float m_run, l_run;
+    int e_out;      /* the values' power of two in O */
+    int lr, g, last, low, hh;
+    bool there, on, wave_on;
+    const char *key_at, *value_at;
+    uint32_t key_x, value_x;
+
+    template <bool RUN>
+    __device__ __forceinline__ void init(const attend_args& a, const attend_row* srow, int n_rows, const char* sk, const char* sv) {
+        const int lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv, col = 32 * (int)(threadIdx.x >> 6) + c32;
+        hh = lane >> 5;
+        lr = col / G;
+        g = col - lr * G;
+        there = lr < n_rows;
+        const attend_row me = srow[there ? lr : 0];
+        last = !there ? -1 : RUN ? me.pos : min(me.shared, me.pos + 1) - 1; /* the last position it may see here */
+        low = a.window ? me.pos - a.window + 1 : INT32_MIN;
+        on = there && last >= 0;
+        wave_on = __any(on);
+        key_at = sk + c32 * HD * 2;
+        key_x = (hh ^ (c32 & (HD / 8 - 1))) << 4; /* piece 2 s + hh: ^ s << 5 */
+        value_at = sv + c32 * 128;
+        value_x = (hh ^ ((c32 >> 1) & 7) ^ (c32 >> 4)) << 4; /* unit 2 s + hh of dimension 32 d + c32: ^ (s ^ d) << 5 */
+        m_run = -INFINITY;
+        l_run = 0.0f;
+        e_out = 126;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) O[d][i] = 0.0f;
+    }
+    /* The queries, through 4 KB of LDS of the wave's own, 32 dimensions at a time: loaded 128 bytes a column (a lane a
+       column would ask for 64 lines an instruction, 18000 cycles a block), taken as operand 16 s + 8 hh .. */
+    __device__ __forceinline__ void load_queries(const attend_args& a, int h, int row0, int n_rows, char* mine) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv;
         float4 in[KS / 2][4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int c = 32 * wave + 8 * i + (lane >> 3), r = min(c / G, n_rows - 1);
-            const float* from_ = a.q + (size_t)(row0 + r) * a.q_stride + (size_t)(h * G + c % G) * HD + 4 * (lane & 7);
+            const float* from = a.q + (size_t)(row0 + r) * a.q_stride + (size_t)(h * G + c % G) * HD + 4 * (lane & 7);
 #pragma unroll
-            for (int t = 0; t < KS / 2; t++) in[t][i] = *reinterpret_cast<const float4*>(from_ + 32 * t);
+            for (int t = 0; t < KS / 2; t++) in[t][i] = *reinterpret_cast<const float4*>(from + 32 * t);
         }
         /* a column's largest magnitude, from its eight lanes to its two */
         uint32_t mag = 0;
@@ -528,7 +632,6 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
         const int k = to_half_range(mag);
         const float f = two_to(k);
         to_score = a.scale * 1.44269504088896340736f * two_to(-k);
-        char* mine = sk + wave * 4096;
 #pragma unroll
         for (int t = 0; t < KS / 2; t++) {
 #pragma unroll
@@ -552,285 +655,342 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
-    const char* key_at = sk + c32 * HD * 2;
-    const uint32_t key_x = (hh ^ (c32 & (HD / 8 - 1))) << 4; /* piece 2 s + hh: ^ s << 5 */
-    const char* value_at = sv + c32 * 128;
-    const uint32_t value_x = (hh ^ ((c32 >> 1) & 7) ^ (c32 >> 4)) << 4; /* unit 2 s + hh of dimension 32 d + c32: ^ (s ^ d) << 5 */
-    float m_run = -INFINITY, l_run = 0.0f;
-    int e_run = 126, e_out = 126; /* the values' power of two, of the block and in this wave's O */
-    f16v O[DT];
+    /* S: sums of products of the keys in LDS; lane: positions 32 pt + 8 (i / 4) + 4 hh + i % 4 of its column */
+    __device__ __forceinline__ void scores() {
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+        for (int pt = 0; pt < 2; pt++) {
+            f16v acc;
 #pragma unroll
-        for (int i = 0; i < 16; i++) O[d][i] = 0.0f;
-
-    const T* kh = (const T*)a.k + (size_t)h * a.head_stride;
-    const T* vh = (const T*)a.v + (size_t)h * a.head_stride;
-    const uint32_t pos_bytes = (uint32_t)(a.pos_stride * sizeof(T)); /* 64 of them stay within 31 bits */
-    const bool on = there && last >= 0, wave_on = __any(on);
-    const T* ks = kh + (size_t)seq * a.seq_stride;
-    const T* vs = vh + (size_t)seq * a.seq_stride;
-    {
-        auto start = [&](int c) { return c < n_sink ? 64 * c : from + 64 * (c - n_sink); };
-        auto stop = [&](int c) { return c < n_sink ? sink : end; };
-        vec<T, 4> rk[U][4], rv[U][4];
-        /* (positions behind the chunk's end read its last again: their scores are masked) */
-        auto fetch = [&](const T* src, int c, vec<T, 4> (&x)[U][4]) {
-            const int t0 = start(c);
-            const uint32_t most = (uint32_t)(min(stop(c) - t0, 64) - 1);
-            const char* from_ = reinterpret_cast<const char*>(src + (size_t)t0 * a.pos_stride);
+            for (int i = 0; i < 16; i++) acc[i] = 0.0f;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int at = tid + sh::NT * u, pg = at / CC, cc = at % CC;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    x[u][i] = *reinterpret_cast<const vec<T, 4>*>(from_ + (min((uint32_t)(4 * pg + i), most) * pos_bytes + (uint32_t)(4 * sizeof(T)) * cc));
-            }
-        };
-        auto publish = [&](const vec<T, 4> (&x)[U][4], uint32_t* to) {
-            uint32_t mag = 0;
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) mag = max(mag, magnitude((float)x[u][i][d]));
-            mag = wave_umax(mag);
-            if (lane == 0) to[wave] = mag;
-        };
-        auto largest = [&](const uint32_t* from_) {
-            uint32_t mag = from_[0];
-#pragma unroll
-            for (int w = 1; w < NW; w++) mag = max(mag, from_[w]);
-            return (uint32_t)__builtin_amdgcn_readfirstlane((int)mag);
-        };
-        /* the finite values' largest magnitude, where some are not: a rare way round, of the whole block */
-        auto finite_largest = [&](const vec<T, 4> (&x)[U][4], uint32_t* slots) {
-            uint32_t mag = 0;
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        const uint32_t v = magnitude((float)x[u][i][d]);
-                        mag = max(mag, v >= MAG_INF ? 0u : v);
-                    }
-            mag = wave_umax(mag);
-            lds_barrier(); /* every wave has read the slots */
-            if (lane == 0) slots[wave] = mag;
-            lds_barrier();
-            return largest(slots);
-        };
-        fetch(ks, c0, rk);
-        fetch(vs, c0, rv);
-        publish(rk, smax);
-        lds_barrier();
-        for (int c = c0; c < c1; c++) {
-            const int t0 = start(c), t1 = stop(c);
-            /* keys to LDS; every wave is past the last chunk's scores */
-            float from_keys = to_score;
-            {
-                float f = 1.0f;
-                if constexpr (SCALED) {
-                    uint32_t mag = largest(smax);
-                    if (__builtin_expect(mag >= MAG_INF, 0)) mag = finite_largest(rk, smax);
-                    const int k = to_half_range(mag);
-                    f = two_to(k);
-                    from_keys = fmaxf(to_score * two_to(-k), 1e-37f); /* (a masked score's -inf times 0 would be NaN) */
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int at = tid + sh::NT * u, pg = at / CC, cc = at % CC;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t to = (key_to(pg, cc) ^ (i << 4)) + i * HD * 2;
-                        uint2 hi, lo;
-                        if constexpr (SCALED) {
-                            cut4((float)rk[u][i][0], (float)rk[u][i][1], (float)rk[u][i][2], (float)rk[u][i][3], f, hi, lo);
-                        } else {
-                            hi = __builtin_bit_cast(uint2, rk[u][i]);
-                        }
-                        *reinterpret_cast<uint2*>(sk + to) = hi;
-                        if constexpr (PARTS) *reinterpret_cast<uint2*>(sk + HALF * 2 + to) = lo;
-                    }
+            for (int s = 0; s < KS; s++) {
+                const char* at = key_at + (key_x ^ (s << 5)) + 32 * pt * HD * 2;
+                const h8v k8 = *reinterpret_cast<const h8v*>(at);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[s], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[s], acc, 0, 0, 0);
+                if constexpr (PARTS) {
+                    const h8v kl = *reinterpret_cast<const h8v*>(at + LO);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[s], acc, 0, 0, 0);
                 }
             }
-            publish(rv, smax + NW);
-            if (c + 1 < c1) fetch(ks, c + 1, rk);
-            lds_barrier();
-            f16v S[2];
-            if (wave_on) {
+            S[pt] = acc;
+        }
+    }
+    /* S from sums to weights of positions t0 .. t1 - 1, 2^(14 + down) exp2(score - maximum) (down <= 0), O and the sum
+       rescaled; from_keys: to_score with the keys' power of two; e: the values' power of two in LDS, less down; bad:
+       null, or the positions whose values are no numbers */
+    __device__ __forceinline__ void weights(const attend_args& a, int t0, int t1, float from_keys, int e, int down, const uint32_t* bad) {
+        from_keys = fmaxf(from_keys, 1e-37f); /* (a masked score's -inf times 0 would be NaN) */
+        const bool whole = !__any(on && !(t0 + 64 <= t1 && t0 + 63 <= last && (t0 >= low || t0 + 64 <= a.sinks))) && __all(on);
+        if (!whole) {
+            /* of the lane's positions, t0 + 4 hh + 32 pt + 8 (i / 4) + i % 4 */
+            const int to_last = on ? min(last, t1 - 1) - t0 - 4 * hh : -1, to_low = max(low, -1) - t0 - 4 * hh, to_sink = a.sinks - t0 - 4 * hh;
 #pragma unroll
-                for (int pt = 0; pt < 2; pt++) {
-                    f16v acc;
+            for (int pt = 0; pt < 2; pt++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) acc[i] = 0.0f;
+                for (int i = 0; i < 16; i++) {
+                    const int t = 32 * pt + 8 * (i >> 2) + (i & 3);
+                    const bool sees = t <= to_last && (t >= to_low || t < to_sink);
+                    S[pt][i] = sees ? S[pt][i] : -INFINITY;
+                }
+        }
+        float m = -INFINITY;
 #pragma unroll
-                    for (int s = 0; s < KS; s++) {
-                        const char* at = key_at + (key_x ^ (s << 5)) + 32 * pt * HD * 2;
-                        const h8v k8 = *reinterpret_cast<const h8v*>(at);
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[s], acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[s], acc, 0, 0, 0);
-                        if constexpr (PARTS) {
-                            const h8v kl = *reinterpret_cast<const h8v*>(at + HALF * 2);
-                            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[s], acc, 0, 0, 0);
-                        }
-                    }
-                    S[pt] = acc;
+        for (int pt = 0; pt < 2; pt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) m = fmaxf(m, S[pt][i]);
+        m = fmaxf(m, __shfl_xor(m, 32, WAVE));
+        m = fmaxf(m_run, m * from_keys);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float f = exp2_hw(m_run - base);
+        const float up = (float)(14 + down) - base;
+        float l = 0.0f;
+        if (__builtin_expect(bad != nullptr, 0)) {
+            for (int pt = 0; pt < 2; pt++) {
+                const uint32_t poison = bad[pt];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float x = pt ? S[1][i] : S[0][i];
+                    if (((poison >> (8 * (i >> 2) + 4 * hh + (i & 3))) & 1) && !(x == -INFINITY)) l = NAN;
                 }
             }
-            /* the values' power of two */
-            float to_half = 1.0f;
-            uint32_t mag = largest(smax + NW);
-            const bool bad = mag >= MAG_INF;
-            if (__builtin_expect(bad, 0)) {
-                mag = finite_largest(rv, smax + NW);
+        }
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int pg = (tid + sh::NT * u) / CC;
+        for (int pt = 0; pt < 2; pt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        bool b = false;
-#pragma unroll
-                        for (int d = 0; d < 4; d++)
-                            if (magnitude((float)rv[u][i][d]) >= MAG_INF) {
-                                rv[u][i][d] = (T)0.0f;
-                                b = true;
-                            }
-                        if (b) atomicOr(&sbad[(4 * pg + i) >> 5], 1u << ((4 * pg + i) & 31));
-                    }
-                }
-                lds_barrier();
+            for (int i = 0; i < 16; i++) {
+                S[pt][i] = exp2_hw(fmaf(S[pt][i], from_keys, up));
+                l += S[pt][i];
             }
-            if constexpr (SCALED) {
-                e_run = min(e_run, to_half_range(mag));
-                to_half = two_to(e_run);
-            }
-            if (wave_on) {
-                /* lane: positions t0 + 32 pt + 8 (i / 4) + 4 hh + i % 4 of its column */
-                const bool whole = !__any(on && !(t0 + 64 <= t1 && t0 + 63 <= last && (t0 >= low || t0 + 64 <= a.sinks))) && __all(on);
-                if (!whole) {
-                    /* of the lane's positions, t0 + 4 hh + 32 pt + 8 (i / 4) + i % 4 */
-                    const int to_last = on ? min(last, t1 - 1) - t0 - 4 * hh : -1, to_low = max(low, -1) - t0 - 4 * hh, to_sink = a.sinks - t0 - 4 * hh;
+        if (down) l *= two_to(min(-down, 126));
+        l_run = fmaf(l_run, f, l);
+        m_run = m;
+        if constexpr (SCALED) {
+            f *= two_to(max(e - e_out, -126));
+            e_out = e;
+        }
+        if (__any(f != 1.0f)) {
 #pragma unroll
-                    for (int pt = 0; pt < 2; pt++)
+            for (int d = 0; d < DT; d++)
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int t = 32 * pt + 8 * (i >> 2) + (i & 3);
-                            const bool sees = t <= to_last && (t >= to_low || t < to_sink);
-                            S[pt][i] = sees ? S[pt][i] : -INFINITY;
-                        }
-                }
-                float m = -INFINITY;
+                for (int i = 0; i < 16; i++) O[d][i] *= f;
+        }
+    }
+    /* O += weights of the values in LDS */
+    __device__ __forceinline__ void values() {
 #pragma unroll
-                for (int pt = 0; pt < 2; pt++)
+        for (int s = 0; s < 4; s++) {
+            /* positions 16 s + 8 (j / 4) + 4 hh + j % 4 as the MFMA's eight, on both operands */
+            const f16v& P = S[s >> 1];
+            const int o = 8 * (s & 1);
+            uint2 h0, l0, h1, l1;
+            cut4(P[o], P[o + 1], P[o + 2], P[o + 3], h0, l0);
+            cut4(P[o + 4], P[o + 5], P[o + 6], P[o + 7], h1, l1);
+            const h8v ph = __builtin_bit_cast(h8v, u32x4{h0.x, h0.y, h1.x, h1.y}), pl = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
 #pragma unroll
-                    for (int i = 0; i < 16; i++) m = fmaxf(m, S[pt][i]);
-                m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-                m = fmaxf(m_run, m * from_keys);
-                const float base = m == -INFINITY ? 0.0f : m;
-                float f = exp2_hw(m_run - base);
-                const float up = 14.0f - base; /* weights up to 2^14 */
-                float l = 0.0f;
-                if (__builtin_expect(bad, 0)) {
-                    for (int pt = 0; pt < 2; pt++) {
-                        const uint32_t poison = sbad[pt];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float x = pt ? S[1][i] : S[0][i];
-                            if (((poison >> (8 * (i >> 2) + 4 * hh + (i & 3))) & 1) && !(x == -INFINITY)) l = NAN;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int pt = 0; pt < 2; pt++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        S[pt][i] = exp2_hw(fmaf(S[pt][i], from_keys, up));
-                        l += S[pt][i];
-                    }
-                l_run = fmaf(l_run, f, l);
-                m_run = m;
-                if constexpr (SCALED) {
-                    f *= two_to(max(e_run - e_out, -126));
-                    e_out = e_run;
-                }
-                if (__any(f != 1.0f)) {
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) O[d][i] *= f;
-                }
-            }
-            /* values to LDS, four positions of a dimension together; every wave is past the last chunk's values */
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int at = tid + sh::NT * u, pg = at / CC, cc = at % CC;
-#pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    const uint32_t to = (value_to(pg, cc) ^ ((d >> 1) << 4)) + d * 128;
-                    uint2 hi, lo;
-                    if constexpr (SCALED) {
-                        cut4((float)rv[u][0][d], (float)rv[u][1][d], (float)rv[u][2][d], (float)rv[u][3][d], to_half, hi, lo);
-                    } else {
-                        hi = __builtin_bit_cast(uint2, vec<T, 4>{rv[u][0][d], rv[u][1][d], rv[u][2][d], rv[u][3][d]});
-                    }
-                    *reinterpret_cast<uint2*>(sv + to) = hi;
-                    if constexpr (PARTS) *reinterpret_cast<uint2*>(sv + HALF * 2 + to) = lo;
-                }
-            }
-            if constexpr (SCALED) {
-                if (c + 1 < c1) publish(rk, smax);
-            }
-            if (c + 1 < c1) fetch(vs, c + 1, rv);
-            lds_barrier();
-            if (bad && tid < 2) sbad[tid] = 0; /* read before this barrier, next written behind another */
-            if (wave_on) {
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    /* positions 16 s + 8 (j / 4) + 4 hh + j % 4 as the MFMA's eight, on both operands */
-                    const f16v& P = S[s >> 1];
-                    const int o = 8 * (s & 1);
-                    uint2 h0, l0, h1, l1;
-                    cut4(P[o], P[o + 1], P[o + 2], P[o + 3], h0, l0);
-                    cut4(P[o + 4], P[o + 5], P[o + 6], P[o + 7], h1, l1);
-                    const h8v ph = __builtin_bit_cast(h8v, u32x4{h0.x, h0.y, h1.x, h1.y}), pl = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const char* at = value_at + (value_x ^ ((s ^ d) << 5)) + 32 * d * 128;
-                        const h8v v8 = *reinterpret_cast<const h8v*>(at);
-                        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, O[d], 0, 0, 0);
-                        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, O[d], 0, 0, 0);
-                        if constexpr (PARTS) {
-                            const h8v vl = *reinterpret_cast<const h8v*>(at + HALF * 2);
-                            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, O[d], 0, 0, 0);
-                        }
-                    }
+            for (int d = 0; d < DT; d++) {
+                const char* at = value_at + (value_x ^ ((s ^ d) << 5)) + 32 * d * 128;
+                const h8v v8 = *reinterpret_cast<const h8v*>(at);
+                O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, O[d], 0, 0, 0);
+                O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, O[d], 0, 0, 0);
+                if constexpr (PARTS) {
+                    const h8v vl = *reinterpret_cast<const h8v*>(at + LO);
+                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, O[d], 0, 0, 0);
                 }
             }
         }
     }
-
-    l_run += __shfl_xor(l_run, 32, WAVE);
-    if (!there) return;
-    const float back = SCALED ? two_to(-e_out) : 1.0f;
-    float* to;
-    float f;
-    if (S == 1) {
-        to = a.out + row * a.out_stride + (size_t)(h * G + g) * HD;
-        f = l_run == 0.0f ? 0.0f : back / l_run;
-    } else {
-        if (hh == 0) p.ml[part] = make_float2(m_run, l_run * 0x1p-14f);
-        if (l_run == 0.0f) return;
-        to = p.acc + part * HD;
-        f = back * 0x1p-14f;
+    __device__ __forceinline__ void flush(const attend_args& a, const attend_parts& p, int split, int h, int row0) {
+        l_run += __shfl_xor(l_run, 32, WAVE);
+        if (!there) return;
+        const int S_ = p.own + p.tile, G = a.n_heads / a.n_kv;
+        const size_t row = (size_t)(row0 + lr), part = ((row * a.n_kv + h) * S_ + p.own + split) * G + g;
+        const float back = SCALED ? two_to(-e_out) : 1.0f;
+        float* to;
+        float f;
+        if (S_ == 1) {
+            to = a.out + row * a.out_stride + (size_t)(h * G + g) * HD;
+            f = l_run == 0.0f ? 0.0f : back / l_run;
+        } else {
+            if (hh == 0) p.ml[part] = make_float2(m_run, l_run * 0x1p-14f);
+            if (l_run == 0.0f) return;
+            to = p.acc + part * HD;
+            f = back * 0x1p-14f;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<float4*>(to + 32 * d + 8 * i + 4 * hh) = make_float4(O[d][4 * i] * f, O[d][4 * i + 1] * f, O[d][4 * i + 2] * f, O[d][4 * i + 3] * f);
     }
+};
+
+/* Split split of what the columns of rows row0 + 0 .. n_rows - 1 see together: RUN, rows of one sequence, each up to itself;
+   otherwise a group's shared prefix. srow are the rows. */
+template <int HD, typename T, int NW, bool RUN>
+__device__ __forceinline__ void group_part(const attend_args& a, const attend_parts& p, int split, int h, int row0, int n_rows,
+                                           const attend_row* srow, const group_span& s, char* lds) {
+    typedef tile_shape<HD, T, NW> sh;
+    typedef chunk_share<HD, T, 64 * NW> share;
+    const int tid = threadIdx.x;
+    uint32_t* smax = reinterpret_cast<uint32_t*>(lds); /* [2][NW]: magnitudes of keys, of values */
+    uint32_t* sbad = smax + 2 * NW;                    /* positions whose values are not finite */
+    char* sk = lds + sh::HEAD;
+    char* sv = sk + (sh::PARTS ? 2 : 1) * sh::HALF * 2;
+    /* seen, in chunks of 64 */
+    const int n_sink = (s.sink + 63) >> 6, n_chunks = n_sink + ((s.end - s.from + 63) >> 6);
+    const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
+    wave_columns<HD, T> w;
+    w.template init<RUN>(a, srow, n_rows, sk, sv);
+    if (c0 < c1) {
+        if (tid < 2) sbad[tid] = 0;
+        w.load_queries(a, h, row0, n_rows, sk + (tid >> 6) * 4096);
+        const T* ks = (const T*)a.k + (size_t)h * a.head_stride + (size_t)s.seq * a.seq_stride;
+        const T* vs = (const T*)a.v + (size_t)h * a.head_stride + (size_t)s.seq * a.seq_stride;
+        auto start = [&](int c) { return c < n_sink ? 64 * c : s.from + 64 * (c - n_sink); };
+        auto stop = [&](int c) { return c < n_sink ? s.sink : s.end; };
+        int e_run = 126; /* the values' power of two, the least so far */
+        share rk, rv;
+        rk.fetch(ks, a.pos_stride, start(c0), stop(c0));
+        rv.fetch(vs, a.pos_stride, start(c0), stop(c0));
+        rk.publish(smax);
+        lds_barrier();
+        for (int c = c0; c < c1; c++) {
+            const int t0 = start(c), t1 = stop(c);
+            /* keys to LDS; every wave is past the last chunk's scores */
+            float from_keys = w.to_score, f = 1.0f;
+            if constexpr (sh::SCALED) {
+                uint32_t mag = share::largest(smax);
+                if (__builtin_expect(mag >= MAG_INF, 0)) mag = rk.finite_largest(smax);
+                const int k = to_half_range(mag);
+                f = two_to(k);
+                from_keys *= two_to(-k);
+            }
+            rk.store_keys(sk, f);
+            rv.publish(smax + NW);
+            if (c + 1 < c1) rk.fetch(ks, a.pos_stride, start(c + 1), stop(c + 1));
+            lds_barrier();
+            if (w.wave_on) w.scores();
+            uint32_t mag = share::largest(smax + NW);
+            const bool bad = mag >= MAG_INF;
+            if (__builtin_expect(bad, 0)) {
+                mag = rv.finite_largest(smax + NW);
+                rv.take_out(sbad);
+                lds_barrier();
+            }
+            if constexpr (sh::SCALED) e_run = min(e_run, to_half_range(mag));
+            if (w.wave_on) w.weights(a, t0, t1, from_keys, e_run, 0, bad ? sbad : nullptr);
+            /* values to LDS; every wave is past the last chunk's values */
+            rv.store_values(sv, sh::SCALED ? two_to(e_run) : 1.0f);
+            if constexpr (sh::SCALED) {
+                if (c + 1 < c1) rk.publish(smax);
+            }
+            if (c + 1 < c1) rv.fetch(vs, a.pos_stride, start(c + 1), stop(c + 1));
+            lds_barrier();
+            if (bad && tid < 2) sbad[tid] = 0; /* read before this barrier, next written behind another */
+            if (w.wave_on) w.values();
+        }
+    }
+    w.flush(a, p, split, h, row0);
+}
+
+/* ---- a prompt's chunk over images of the cache ----
+   Cutting 64 positions into parts is as much vector work as one wave's products with them is matrix work, and every tile of
+   rows repeats it, in step with its barriers. Where many tiles read the same positions they are cut once, into images of what
+   the LDS then holds, and a tile's block only copies: the next keys under this chunk's weighted values, the values under
+   its scores. Blocks of four waves then need half the LDS and registers, and the two of a compute unit fill each other's
+   gaps. */
+#define IMAGE_WAVES 4
+template <int HD, typename T>
+constexpr size_t image_part_bytes = (sizeof(T) == 4 ? 2 : 1) * 64 * HD * 2; /* the keys', and the values' behind them */
+
+/* Chunk c (positions 64 c ..) lies in slot c (c < x) or c - y. */
+__device__ __forceinline__ int2 image_slots(const attend_args& a, uint32_t far, uint32_t near) {
+    const int end = min((int)far, a.ctx), least = near ? (int)(0x80000000u - near) : 0;
+    const int sink = a.window ? min(a.sinks, end) : 0, from = a.window ? min(max(sink, least - a.window + 1), end) : 0;
+    const int n_sink = (sink + 63) >> 6;
+    return make_int2(n_sink, max(n_sink, from >> 6) - n_sink);
+}
+
+template <int HD, typename T>
+__global__ __launch_bounds__(256) void attend_image_kernel(attend_args a, attend_parts p) {
+    typedef chunk_share<HD, T, 256> share;
+    constexpr size_t PART = image_part_bytes<HD, T>;
+    __shared__ __attribute__((aligned(16))) char image[2 * PART];
+    __shared__ uint32_t smax[2][4], sbad[2];
+    const int tid = threadIdx.x, wave = tid >> 6, h = blockIdx.x % a.n_kv, slot = blockIdx.x / a.n_kv;
+    /* the run's furthest and nearest positions */
+    uint32_t far = 0, near = 0;
+    int seq = a.run_seq;
+    if (a.recs) {
+        for (int i = tid; i < a.n; i += 256) {
+            const attend_row r = row_of(a, i);
+            if (r.pos >= 0) {
+                far = max(far, (uint32_t)r.pos + 1);
+                near = max(near, 0x80000000u - (uint32_t)r.pos);
+            }
+        }
+        far = wave_umax(far);
+        near = wave_umax(near);
+        if ((tid & 63) == 0) { smax[0][wave] = far; smax[1][wave] = near; }
+        __syncthreads();
+        far = share::largest(smax[0]);
+        near = share::largest(smax[1]);
+        seq = row_of(a, 0).seq;
+        __syncthreads();
+    } else {
+        far = a.run_pos + a.n;
+        near = 0x80000000u - (uint32_t)a.run_pos;
+    }
+    if (tid < 2) sbad[tid] = 0;
+    const int2 at = image_slots(a, far, near);
+    if (blockIdx.x == 0 && tid == 0) p.meta[0] = make_int4(at.x, at.y, 0, 0);
+    const int end = min((int)far, a.ctx), c = slot < at.x ? slot : slot + at.y;
+    if (64 * c >= end) return;
+    const T* ks = (const T*)a.k + (size_t)h * a.head_stride + (size_t)seq * a.seq_stride;
+    const T* vs = (const T*)a.v + (size_t)h * a.head_stride + (size_t)seq * a.seq_stride;
+    share rk, rv;
+    rk.fetch(ks, a.pos_stride, 64 * c, end);
+    rv.fetch(vs, a.pos_stride, 64 * c, end);
+    rk.publish(smax[0]);
+    rv.publish(smax[1]);
+    __syncthreads();
+    uint32_t mk = share::largest(smax[0]), mv = share::largest(smax[1]);
+    if (__builtin_expect(mk >= MAG_INF, 0)) mk = rk.finite_largest(smax[0]);
+    if (__builtin_expect(mv >= MAG_INF, 0)) {
+        mv = rv.finite_largest(smax[1]);
+        rv.take_out(sbad);
+    }
+    const int kk = to_half_range(mk), kv = to_half_range(mv);
+    rk.store_keys(image, two_to(kk));
+    rv.store_values(image + PART, two_to(kv));
+    __syncthreads();
+    const size_t to = (size_t)h * p.slots + slot;
+    u32x4* out = reinterpret_cast<u32x4*>(p.images + to * 2 * PART);
+    for (int i = tid; i < (int)(2 * PART / 16); i += 256) out[i] = reinterpret_cast<const u32x4*>(image)[i];
+    if (tid == 0) p.meta[1 + to] = make_int4(kk, kv, (int)sbad[0], (int)sbad[1]);
+}
+
+/* A wave's share of BYTES to LDS, asked for; image_wait waits for all waves'. */
+template <int BYTES>
+__device__ __forceinline__ void image_load(const char* from, char* to) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            *reinterpret_cast<float4*>(to + 32 * d + 8 * i + 4 * hh) = make_float4(O[d][4 * i] * f, O[d][4 * i + 1] * f, O[d][4 * i + 2] * f, O[d][4 * i + 3] * f);
+    for (int j = 0; j < BYTES / 1024 / IMAGE_WAVES; j++) {
+        const int at = (j * IMAGE_WAVES + wave) * 1024;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + at + 16 * lane),
+                                         (__attribute__((address_space(3))) void*)(to + at), 16, 0, 0);
+    }
+}
+__device__ __forceinline__ void image_wait() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+}
+
+template <int HD, typename T>
+__global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_imaged_kernel(attend_args a, attend_parts p) {
+    constexpr int PART = (int)image_part_bytes<HD, T>;
+    constexpr bool SCALED = wave_columns<HD, T>::SCALED;
+    __shared__ __attribute__((aligned(1024))) char sk[PART > IMAGE_WAVES * 4096 ? PART : IMAGE_WAVES * 4096]; /* (the queries pass through it) */
+    __shared__ __attribute__((aligned(1024))) char sv[PART];
+    __shared__ attend_row srow[32 * IMAGE_WAVES];
+    const int tid = threadIdx.x, split = blockIdx.y, h = blockIdx.x % a.n_kv, G = a.n_heads / a.n_kv, TR = 32 * IMAGE_WAVES / G;
+    const int r0 = blockIdx.x / a.n_kv * TR, nr = min(TR, a.n - r0);
+    load_rows<64 * IMAGE_WAVES>(a, r0, nr, srow);
+    lds_barrier();
+    const group_span s = group_seen<true>(a, srow, 0, nr);
+    const int4 at = p.meta[0];
+    /* seen, in chunks of 64 positions: c < n_sink, and from first on */
+    const int n_sink = (s.sink + 63) >> 6, first = max(n_sink, s.from >> 6), n_chunks = n_sink + max(((s.end + 63) >> 6) - first, 0);
+    const int per = (n_chunks + p.tile - 1) / p.tile, i0 = split * per, i1 = min(i0 + per, n_chunks);
+    wave_columns<HD, T> w;
+    w.template init<true>(a, srow, nr, sk, sv);
+    if (i0 < i1) {
+        w.load_queries(a, h, r0, nr, sk + (tid >> 6) * 4096);
+        const char* images = p.images + (size_t)h * p.slots * 2 * PART;
+        const int4* meta = p.meta + 1 + (size_t)h * p.slots;
+        auto chunk = [&](int i) { return i < n_sink ? i : first + (i - n_sink); };
+        auto slot = [&](int i) { const int c = chunk(i); return c < at.x ? c : c - at.y; };
+        int e_run = 126;
+        lds_barrier(); /* every wave has its queries */
+        image_load<PART>(images + (size_t)slot(i0) * 2 * PART, sk);
+        for (int i = i0; i < i1; i++) {
+            const int4 m = meta[slot(i)];
+            image_wait(); /* the keys are there; every wave is past the last chunk's values */
+            image_load<PART>(images + ((size_t)slot(i) * 2 + 1) * PART, sv);
+            if (w.wave_on) {
+                w.scores();
+                if constexpr (SCALED) e_run = min(e_run, m.y);
+                const bool bad = (m.z | m.w) != 0;
+                w.weights(a, 64 * chunk(i), s.end, SCALED ? w.to_score * two_to(-m.x) : w.to_score, e_run, SCALED ? e_run - m.y : 0,
+                          bad ? reinterpret_cast<const uint32_t*>(&meta[slot(i)].z) : nullptr);
+            }
+            image_wait(); /* the values are there; every wave is past the keys */
+            if (i + 1 < i1) image_load<PART>(images + (size_t)slot(i + 1) * 2 * PART, sk);
+            if (w.wave_on) w.values();
+        }
+    }
+    w.flush(a, p, split, h, r0);
 }
 
 /* Split split of a tile's rows: RUN all together, otherwise its groups of many columns, one after another. */
@@ -961,6 +1121,10 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(attend_args a, attend
     if (head < a.n_heads) reinterpret_cast<float4*>(a.out + (size_t)row * a.out_stride + (size_t)head * HD)[d] = o;
 }
 
+/* A run of so many tiles or more goes over images, if they take no more bytes than this. */
+#define IMAGE_TILES 8
+#define IMAGE_BYTES_MAX ((size_t)256 << 20)
+
 /* How a call is cut into blocks. */
 static attend_parts plan(const attend_args& a) {
     attend_parts p = {};
@@ -969,6 +1133,18 @@ static attend_parts plan(const attend_args& a) {
     const long seen = a.window ? std::min<long>(a.own_max, (long)a.window + a.sinks) : a.own_max;
     const long blocks = 256; /* a block a compute unit */
     if (a.run) {
+        const int few_rows = 32 * IMAGE_WAVES / G, few_tiles = (a.n + few_rows - 1) / few_rows;
+        /* the images' slots: consecutive rows see window + n positions and the sinks */
+        const long reach = (a.own_max + 63) / 64 + 1, near = a.window ? (std::min(a.sinks, a.own_max) + 63) / 64 + ((long)a.window + a.n + 63) / 64 + 2 : reach;
+        const long slots = a.recs ? reach : std::min(reach, near);
+        const size_t bytes = (size_t)slots * a.n_kv * 2 * 64 * a.hd * 2 * (a.dtype == VITNA_DTYPE_F32 ? 2 : 1);
+        if (few_tiles >= IMAGE_TILES && bytes <= IMAGE_BYTES_MAX) {
+            const long per_tile = (a.window ? std::min<long>(a.own_max, (long)a.window + a.sinks + few_rows) : a.own_max) / 64 + 2;
+            p.tiles = few_tiles;
+            p.slots = (int)slots;
+            p.tile = (int)std::min<long>(std::min<long>(per_tile, 64), std::max<long>(1, 2 * blocks / ((long)few_tiles * a.n_kv)));
+            return p;
+        }
         const long chunks = (a.window ? std::min<long>(a.own_max, (long)a.window + a.sinks + rows) : a.own_max) / 64 + 1;
         p.tile = (int)std::min<long>(std::min<long>(chunks, 64), std::max<long>(1, blocks / ((long)p.tiles * a.n_kv)));
         return p;
@@ -984,22 +1160,31 @@ static attend_parts plan(const attend_args& a) {
     return p;
 }
 
-static size_t parts_bytes(const attend_args& a, const attend_parts& p, size_t* acc) {
-    const size_t S = (size_t)p.own + p.tile, heads = (size_t)a.n * a.n_heads * S;
-    *acc = align256(heads * sizeof(float2));
-    return S > 1 ? *acc + heads * a.hd * sizeof(float) : 16;
+/* Bytes of work: maxima and sums, values, images and their meta; where they lie in it, into p (base may be null). */
+static size_t place_parts(const attend_args& a, attend_parts& p, char* base) {
+    const size_t S = (size_t)p.own + p.tile, heads = S > 1 ? (size_t)a.n * a.n_heads * S : 0, slots = (size_t)p.slots * a.n_kv;
+    const size_t ml = align256(heads * sizeof(float2)), acc = align256(heads * a.hd * sizeof(float));
+    const size_t meta = p.slots ? align256((1 + slots) * sizeof(int4)) : 0, images = slots * 2 * 64 * a.hd * 2 * (a.dtype == VITNA_DTYPE_F32 ? 2 : 1);
+    p.ml = reinterpret_cast<float2*>(base);
+    p.acc = reinterpret_cast<float*>(base + ml);
+    p.meta = reinterpret_cast<int4*>(base + ml + acc);
+    p.images = base + ml + acc + meta;
+    return std::max<size_t>(ml + acc + meta + images, 16);
 }
 
 size_t attend_work(const attend_args& a) {
-    size_t acc;
-    return parts_bytes(a, plan(a), &acc);
+    attend_parts p = plan(a);
+    return place_parts(a, p, nullptr);
 }
 
 template <int HD, typename T>
 static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_t s) {
     constexpr int NW = tile_waves<HD>;
     const unsigned heads = (unsigned)a.n_kv;
-    if (a.run) {
+    if (p.slots) {
+        attend_image_kernel<HD, T><<<p.slots * heads, 256, 0, s>>>(a, p);
+        attend_imaged_kernel<HD, T><<<dim3(p.tiles * heads, p.tile), 64 * IMAGE_WAVES, 0, s>>>(a, p);
+    } else if (a.run) {
         attend_tile_kernel<HD, T, true><<<dim3(p.tiles * heads, p.tile), 64 * NW, 0, s>>>(a, p);
     } else if (p.tile) {
         attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.tile + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
@@ -1020,11 +1205,8 @@ static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_
 hipError_t launch_attend(const attend_args& a, hipStream_t s) {
     if (a.n < 1 || a.n_kv < 1 || a.n_heads % a.n_kv || a.n_heads / a.n_kv > ATTEND_G_MAX) return hipErrorInvalidValue;
     attend_parts p = plan(a);
-    size_t acc;
-    if (parts_bytes(a, p, &acc) > a.work_bytes || p.own + p.tile > MERGE_SPLITS) return hipErrorInvalidValue;
+    if (place_parts(a, p, static_cast<char*>(a.work)) > a.work_bytes || p.own + p.tile > MERGE_SPLITS) return hipErrorInvalidValue;
     if ((long)a.n * a.n_kv > (1L << 22)) return hipErrorInvalidValue; /* threads of a launch stay within 32 bits */
-    p.ml = static_cast<float2*>(a.work);
-    p.acc = reinterpret_cast<float*>(static_cast<char*>(a.work) + acc);
     if (a.hd == 128) {
         if (a.dtype == VITNA_DTYPE_F32) return launch<128, float>(a, p, s);
         if (a.dtype == VITNA_DTYPE_F16) return launch<128, _Float16>(a, p, s);
