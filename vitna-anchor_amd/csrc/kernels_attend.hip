@@ -34,7 +34,7 @@
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef __fp16 h2v __attribute__((ext_vector_type(2)));
+typedef int int4_ __attribute__((ext_vector_type(4)));
 
 template <typename T, int N>
 struct vec_of {
@@ -439,10 +439,20 @@ __device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, flo
     lo = make_uint2(pack_cut(fmaf(x0, s, -half_lo(hi.x)), fmaf(x1, s, -half_hi(hi.x))), pack_cut(fmaf(x2, s, -half_lo(hi.y)), fmaf(x3, s, -half_hi(hi.y))));
 }
 
+/* x less a half of h: one instruction (the compiler widens the half first) */
+__device__ __forceinline__ float less_lo(float x, uint32_t h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float less_hi(float x, uint32_t h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
 __device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, uint2& hi, uint2& lo) {
     hi = make_uint2(pack_cut(x0, x1), pack_cut(x2, x3));
-    lo = make_uint2(pack_cut(fmaf(half_lo(hi.x), -1.0f, x0), fmaf(half_hi(hi.x), -1.0f, x1)),
-                    pack_cut(fmaf(half_lo(hi.y), -1.0f, x2), fmaf(half_hi(hi.y), -1.0f, x3)));
+    lo = make_uint2(pack_cut(less_lo(x0, hi.x), less_hi(x1, hi.x)), pack_cut(less_lo(x2, hi.y), less_hi(x3, hi.y)));
 }
 
 /* The k of 2^k that brings a magnitude to 2^14 .. 2^15 (0 and numbers near it: as far as 2^k reaches). */
@@ -461,20 +471,23 @@ struct tile_shape {
     static_assert(U >= 1 && U * NT == 16 * CC, "whole groups a thread");
 };
 
-/* Places in a chunk's LDS (and image). Keys [part][64 positions][HD] in pieces of 8 dimensions, piece x of position t at
-   x ^ t mod (HD / 8). Values [part][HD][64 positions] in units of two pieces of 4 positions, those of one MFMA operand
-   (positions 16 s + 4 hh .. and 16 s + 8 + 4 hh ..: unit 2 s + hh), unit x of dimension d at x ^ (d / 2 ^ d / 16) mod 8.
-   Sixteen lanes' 16-byte reads then take every bank once, and all places are one lane's ^ and + a constant. Thread group
-   (pg, cc) holds positions 4 pg + i and dimensions 4 cc + d: key i at (key_to ^ i << 4) + i rows, values d at
-   (value_to ^ (d / 2) << 4) + d rows. */
+/* Places in LDS (and in an image) of POS = 64 or 32 positions. Keys [part][POS][HD] in pieces of 8 dimensions, piece x of
+   position t at x ^ t mod (HD / 8). Values [part][HD][POS] in units of two pieces of 4 positions, those of one MFMA operand
+   (positions 16 s + 4 hh .. and 16 s + 8 + 4 hh ..: unit 2 s + hh), unit x of dimension d at x ^ (d / 2 ^ d / 16) mod 8
+   (POS 32: x ^ d / 4 mod 4). Sixteen lanes' 16-byte reads then take every bank once, and all places are one lane's ^ and +
+   a constant. Thread group (pg, cc) holds positions 4 pg + i and dimensions 4 cc + d: key i at (key_to ^ i << 4) + i rows,
+   values d at (value_to ^ value_swap(d)) + d rows. */
 template <int HD>
 __device__ __forceinline__ uint32_t key_to(int pg, int cc) {
     return (uint32_t)(4 * pg * HD * 2 + (((cc >> 1) ^ ((4 * pg) & (HD / 8 - 1))) << 4) + 8 * (cc & 1));
 }
+template <int POS>
 __device__ __forceinline__ uint32_t value_to(int pg, int cc) {
-    const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1;
-    return (uint32_t)(4 * cc * 128 + ((unit ^ (((2 * cc) ^ (cc >> 2)) & 7)) << 4) + 8 * half);
+    const int unit = 2 * (pg >> 2) + (pg & 1), half = (pg >> 1) & 1, x = POS == 64 ? ((2 * cc) ^ (cc >> 2)) & 7 : cc & 3;
+    return (uint32_t)(4 * cc * POS * 2 + ((unit ^ x) << 4) + 8 * half);
 }
+template <int POS>
+__device__ __forceinline__ constexpr uint32_t value_swap(int d) { return POS == 64 ? (d >> 1) << 4 : 0; }
 
 /* A thread's share of 64 positions' keys or values: U groups of 4 positions x 4 dimensions. */
 template <int HD, typename T, int NT>
@@ -540,39 +553,48 @@ struct chunk_share {
             }
         }
     }
-    __device__ __forceinline__ void store_keys(char* sk, float f) const {
+    /* times f, in parts; POS 32: the second half of the positions next bytes behind the first */
+    template <int POS = 64>
+    __device__ __forceinline__ void store_keys(char* sk, float f, size_t next = 0) const {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int at = threadIdx.x + NT * u, pg = at / CC, cc = at % CC;
+            char* to = sk + (POS == 32 && pg >= 8 ? next : 0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) put(sk + (key_to<HD>(pg, cc) ^ (i << 4)) + i * HD * 2, x[u][i][0], x[u][i][1], x[u][i][2], x[u][i][3], f);
+            for (int i = 0; i < 4; i++) put<POS>(to + (key_to<HD>(pg & (POS / 4 - 1), cc) ^ (i << 4)) + i * HD * 2, x[u][i][0], x[u][i][1], x[u][i][2], x[u][i][3], f);
         }
     }
-    __device__ __forceinline__ void store_values(char* sv, float f) const {
+    template <int POS = 64>
+    __device__ __forceinline__ void store_values(char* sv, float f, size_t next = 0) const {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int at = threadIdx.x + NT * u, pg = at / CC, cc = at % CC;
+            char* to = sv + (POS == 32 && pg >= 8 ? next : 0);
 #pragma unroll
-            for (int d = 0; d < 4; d++) put(sv + (value_to(pg, cc) ^ ((d >> 1) << 4)) + d * 128, x[u][0][d], x[u][1][d], x[u][2][d], x[u][3][d], f);
+            for (int d = 0; d < 4; d++) put<POS>(to + (value_to<POS>(pg & (POS / 4 - 1), cc) ^ value_swap<POS>(d)) + d * POS * 2, x[u][0][d], x[u][1][d], x[u][2][d], x[u][3][d], f);
         }
     }
+    template <int POS>
     static __device__ __forceinline__ void put(char* to, T a, T b, T c, T d, float f) {
         uint2 hi, lo;
         if constexpr (std::is_same<T, _Float16>::value) hi = __builtin_bit_cast(uint2, vec<T, 4>{a, b, c, d});
         else cut4((float)a, (float)b, (float)c, (float)d, f, hi, lo);
         *reinterpret_cast<uint2*>(to) = hi;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(to + 64 * HD * 2) = lo;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint2*>(to + POS * HD * 2) = lo;
     }
 };
 
+#define WEIGHT_EXP 6
+#define WEIGHT_SLACK 8.0f
+
 /* A wave's 32 columns: queries, running maximum, sum and weighted values. Column 32 wave + c32 is row row0 + x / G, query
    head h G + x mod G; lanes c32 and c32 + 32 hold its halves. */
-template <int HD, typename T>
+template <int HD, typename T, int POS>
 struct wave_columns {
     static constexpr bool PARTS = sizeof(T) == 4, SCALED = !std::is_same<T, _Float16>::value;
-    static constexpr int KS = HD / 16, DT = HD / 32, LO = 64 * HD * 2; /* bytes from a hi part to its lo part */
+    static constexpr int KS = HD / 16, DT = HD / 32, PT = POS / 32, LO = POS * HD * 2; /* bytes from a hi part to its lo part */
     h8v qh[KS], ql[KS];
-    f16v S[2], O[DT];
+    f16v S[PT], O[DT];
     float to_score; /* from the products' sums to scores in units of log 2, but for the keys' power of two */
     float m_run, l_run;
     int e_out;      /* the values' power of two in O */
@@ -581,6 +603,12 @@ struct wave_columns {
     const char *key_at, *value_at;
     uint32_t key_x, value_x;
 
+    /* the keys and values to work on */
+    __device__ __forceinline__ void at(const char* sk, const char* sv) {
+        const int c32 = threadIdx.x & 31;
+        key_at = sk + c32 * HD * 2;
+        value_at = sv + c32 * POS * 2;
+    }
     template <bool RUN>
     __device__ __forceinline__ void init(const attend_args& a, const attend_row* srow, int n_rows, const char* sk, const char* sv) {
         const int lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv, col = 32 * (int)(threadIdx.x >> 6) + c32;
@@ -593,10 +621,10 @@ struct wave_columns {
         low = a.window ? me.pos - a.window + 1 : INT32_MIN;
         on = there && last >= 0;
         wave_on = __any(on);
-        key_at = sk + c32 * HD * 2;
+        at(sk, sv);
         key_x = (hh ^ (c32 & (HD / 8 - 1))) << 4; /* piece 2 s + hh: ^ s << 5 */
-        value_at = sv + c32 * 128;
-        value_x = (hh ^ ((c32 >> 1) & 7) ^ (c32 >> 4)) << 4; /* unit 2 s + hh of dimension 32 d + c32: ^ (s ^ d) << 5 */
+        /* unit 2 s + hh of dimension 32 d + c32: ^ (s ^ d) << 5 (POS 32: ^ s << 5) */
+        value_x = (POS == 64 ? hh ^ ((c32 >> 1) & 7) ^ (c32 >> 4) : hh ^ ((c32 >> 2) & 3)) << 4;
         m_run = -INFINITY;
         l_run = 0.0f;
         e_out = 126;
@@ -658,7 +686,7 @@ struct wave_columns {
     /* S: sums of products of the keys in LDS; lane: positions 32 pt + 8 (i / 4) + 4 hh + i % 4 of its column */
     __device__ __forceinline__ void scores() {
 #pragma unroll
-        for (int pt = 0; pt < 2; pt++) {
+        for (int pt = 0; pt < PT; pt++) {
             f16v acc;
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[i] = 0.0f;
@@ -676,17 +704,19 @@ struct wave_columns {
             S[pt] = acc;
         }
     }
-    /* S from sums to weights of positions t0 .. t1 - 1, 2^(14 + down) exp2(score - maximum) (down <= 0), O and the sum
-       rescaled; from_keys: to_score with the keys' power of two; e: the values' power of two in LDS, less down; bad:
-       null, or the positions whose values are no numbers */
-    __device__ __forceinline__ void weights(const attend_args& a, int t0, int t1, float from_keys, int e, int down, const uint32_t* bad) {
-        from_keys = fmaxf(from_keys, 1e-37f); /* (a masked score's -inf times 0 would be NaN) */
-        const bool whole = !__any(on && !(t0 + 64 <= t1 && t0 + 63 <= last && (t0 >= low || t0 + 64 <= a.sinks))) && __all(on);
+    /* S from sums to weights of positions t0 .. t1 - 1, 2^(WEIGHT_EXP + down) exp2(score - m_run) (down <= 0). m_run, and
+       with it O and the sum, follows the maximum only where that is WEIGHT_SLACK above it: a weight then is 2^14 at most, as
+       f16 holds, and after a few chunks hardly any rescale O (a wave's 32 columns would at every other). keys: to_score with
+       the keys' power of two; e: the values' power of two in LDS, less down; bad0, bad1: the positions whose values are no
+       numbers. */
+    __device__ __forceinline__ void weights(const attend_args& a, int t0, int t1, float keys, int e, int down, uint32_t bad0, uint32_t bad1) {
+        keys = fmaxf(keys, 1e-37f); /* (a masked score's -inf times 0 would be NaN) */
+        const bool whole = !__any(on && !(t0 + POS <= t1 && t0 + POS - 1 <= last && (t0 >= low || t0 + POS <= a.sinks))) && __all(on);
         if (!whole) {
             /* of the lane's positions, t0 + 4 hh + 32 pt + 8 (i / 4) + i % 4 */
             const int to_last = on ? min(last, t1 - 1) - t0 - 4 * hh : -1, to_low = max(low, -1) - t0 - 4 * hh, to_sink = a.sinks - t0 - 4 * hh;
 #pragma unroll
-            for (int pt = 0; pt < 2; pt++)
+            for (int pt = 0; pt < PT; pt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int t = 32 * pt + 8 * (i >> 2) + (i & 3);
@@ -696,33 +726,33 @@ struct wave_columns {
         }
         float m = -INFINITY;
 #pragma unroll
-        for (int pt = 0; pt < 2; pt++)
+        for (int pt = 0; pt < PT; pt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) m = fmaxf(m, S[pt][i]);
-        m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-        m = fmaxf(m_run, m * from_keys);
+        m = fmaxf(m, __shfl_xor(m, 32, WAVE)) * keys;
+        m = m > m_run + WEIGHT_SLACK ? m : m_run;
         const float base = m == -INFINITY ? 0.0f : m;
-        float f = exp2_hw(m_run - base);
-        const float up = (float)(14 + down) - base;
-        float l = 0.0f;
-        if (__builtin_expect(bad != nullptr, 0)) {
-            for (int pt = 0; pt < 2; pt++) {
-                const uint32_t poison = bad[pt];
+        float f = exp2_hw(m_run - base), l = 0.0f;
+        const float up = (float)(WEIGHT_EXP + down) - base;
+        if (__builtin_expect((bad0 | bad1) != 0, 0)) {
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++) {
+                const uint32_t poison = pt ? bad1 : bad0;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float x = pt ? S[1][i] : S[0][i];
+                    const float x = S[pt][i];
                     if (((poison >> (8 * (i >> 2) + 4 * hh + (i & 3))) & 1) && !(x == -INFINITY)) l = NAN;
                 }
             }
         }
 #pragma unroll
-        for (int pt = 0; pt < 2; pt++)
+        for (int pt = 0; pt < PT; pt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                S[pt][i] = exp2_hw(fmaf(S[pt][i], from_keys, up));
+                S[pt][i] = exp2_hw(fmaf(S[pt][i], keys, up));
                 l += S[pt][i];
             }
-        if (down) l *= two_to(min(-down, 126));
+        l *= two_to(min(-down, 126));
         l_run = fmaf(l_run, f, l);
         m_run = m;
         if constexpr (SCALED) {
@@ -739,7 +769,7 @@ struct wave_columns {
     /* O += weights of the values in LDS */
     __device__ __forceinline__ void values() {
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
+        for (int s = 0; s < POS / 16; s++) {
             /* positions 16 s + 8 (j / 4) + 4 hh + j % 4 as the MFMA's eight, on both operands */
             const f16v& P = S[s >> 1];
             const int o = 8 * (s & 1);
@@ -747,16 +777,21 @@ struct wave_columns {
             cut4(P[o], P[o + 1], P[o + 2], P[o + 3], h0, l0);
             cut4(P[o + 4], P[o + 5], P[o + 6], P[o + 7], h1, l1);
             const h8v ph = __builtin_bit_cast(h8v, u32x4{h0.x, h0.y, h1.x, h1.y}), pl = __builtin_bit_cast(h8v, u32x4{l0.x, l0.y, l1.x, l1.y});
+            h8v v[DT], vl[DT];
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const char* at = value_at + (value_x ^ ((s ^ d) << 5)) + 32 * d * 128;
-                const h8v v8 = *reinterpret_cast<const h8v*>(at);
-                O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, O[d], 0, 0, 0);
-                O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, O[d], 0, 0, 0);
-                if constexpr (PARTS) {
-                    const h8v vl = *reinterpret_cast<const h8v*>(at + LO);
-                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph, O[d], 0, 0, 0);
-                }
+                const char* at = value_at + (value_x ^ ((POS == 64 ? s ^ d : s) << 5)) + 32 * d * POS * 2;
+                v[d] = *reinterpret_cast<const h8v*>(at);
+                if constexpr (PARTS) vl[d] = *reinterpret_cast<const h8v*>(at + LO);
+            }
+            /* one accumulator's products apart */
+#pragma unroll
+            for (int d = 0; d < DT; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph, O[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < DT; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl, O[d], 0, 0, 0);
+            if constexpr (PARTS) {
+#pragma unroll
+                for (int d = 0; d < DT; d++) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl[d], ph, O[d], 0, 0, 0);
             }
         }
     }
@@ -772,10 +807,10 @@ struct wave_columns {
             to = a.out + row * a.out_stride + (size_t)(h * G + g) * HD;
             f = l_run == 0.0f ? 0.0f : back / l_run;
         } else {
-            if (hh == 0) p.ml[part] = make_float2(m_run, l_run * 0x1p-14f);
+            if (hh == 0) p.ml[part] = make_float2(m_run, l_run * two_to(-WEIGHT_EXP));
             if (l_run == 0.0f) return;
             to = p.acc + part * HD;
-            f = back * 0x1p-14f;
+            f = back * two_to(-WEIGHT_EXP);
         }
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -800,7 +835,7 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
     /* seen, in chunks of 64 */
     const int n_sink = (s.sink + 63) >> 6, n_chunks = n_sink + ((s.end - s.from + 63) >> 6);
     const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
-    wave_columns<HD, T> w;
+    wave_columns<HD, T, 64> w;
     w.template init<RUN>(a, srow, n_rows, sk, sv);
     if (c0 < c1) {
         if (tid < 2) sbad[tid] = 0;
@@ -839,7 +874,7 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
                 lds_barrier();
             }
             if constexpr (sh::SCALED) e_run = min(e_run, to_half_range(mag));
-            if (w.wave_on) w.weights(a, t0, t1, from_keys, e_run, 0, bad ? sbad : nullptr);
+            if (w.wave_on) w.weights(a, t0, t1, from_keys, e_run, 0, bad ? sbad[0] : 0, bad ? sbad[1] : 0);
             /* values to LDS; every wave is past the last chunk's values */
             rv.store_values(sv, sh::SCALED ? two_to(e_run) : 1.0f);
             if constexpr (sh::SCALED) {
@@ -857,12 +892,12 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
 /* ---- a prompt's chunk over images of the cache ----
    Cutting 64 positions into parts is as much vector work as one wave's products with them is matrix work, and every tile of
    rows repeats it, in step with its barriers. Where many tiles read the same positions they are cut once, into images of what
-   the LDS then holds, and a tile's block only copies: the next keys under this chunk's weighted values, the values under
-   its scores. Blocks of four waves then need half the LDS and registers, and the two of a compute unit fill each other's
-   gaps. */
+   the LDS then holds, 32 positions each. A tile's block only copies: the next 32 positions while it works on these, so that
+   a copy has the time of 96 products to arrive, and the two blocks of a compute unit (four waves, 64 KB each) fill each
+   other's gaps. */
 #define IMAGE_WAVES 4
 template <int HD, typename T>
-constexpr size_t image_part_bytes = (sizeof(T) == 4 ? 2 : 1) * 64 * HD * 2; /* the keys', and the values' behind them */
+constexpr int image_part = (sizeof(T) == 4 ? 2 : 1) * 32 * HD * 2; /* bytes of 32 positions' keys, and of their values behind them */
 
 /* Chunk c (positions 64 c ..) lies in slot c (c < x) or c - y. */
 __device__ __forceinline__ int2 image_slots(const attend_args& a, uint32_t far, uint32_t near) {
@@ -872,11 +907,12 @@ __device__ __forceinline__ int2 image_slots(const attend_args& a, uint32_t far, 
     return make_int2(n_sink, max(n_sink, from >> 6) - n_sink);
 }
 
+/* Block (key-value head, slot): 64 positions. */
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void attend_image_kernel(attend_args a, attend_parts p) {
     typedef chunk_share<HD, T, 256> share;
-    constexpr size_t PART = image_part_bytes<HD, T>;
-    __shared__ __attribute__((aligned(16))) char image[2 * PART];
+    constexpr int PART = image_part<HD, T>;
+    __shared__ __attribute__((aligned(16))) char image[4 * PART];
     __shared__ uint32_t smax[2][4], sbad[2];
     const int tid = threadIdx.x, wave = tid >> 6, h = blockIdx.x % a.n_kv, slot = blockIdx.x / a.n_kv;
     /* the run's furthest and nearest positions */
@@ -922,12 +958,12 @@ __global__ __launch_bounds__(256) void attend_image_kernel(attend_args a, attend
         rv.take_out(sbad);
     }
     const int kk = to_half_range(mk), kv = to_half_range(mv);
-    rk.store_keys(image, two_to(kk));
-    rv.store_values(image + PART, two_to(kv));
+    rk.template store_keys<32>(image, two_to(kk), 2 * PART);
+    rv.template store_values<32>(image + PART, two_to(kv), 2 * PART);
     __syncthreads();
     const size_t to = (size_t)h * p.slots + slot;
-    u32x4* out = reinterpret_cast<u32x4*>(p.images + to * 2 * PART);
-    for (int i = tid; i < (int)(2 * PART / 16); i += 256) out[i] = reinterpret_cast<const u32x4*>(image)[i];
+    u32x4* out = reinterpret_cast<u32x4*>(p.images + to * 4 * PART);
+    for (int i = tid; i < 4 * PART / 16; i += 256) out[i] = reinterpret_cast<const u32x4*>(image)[i];
     if (tid == 0) p.meta[1 + to] = make_int4(kk, kv, (int)sbad[0], (int)sbad[1]);
 }
 
@@ -949,10 +985,11 @@ __device__ __forceinline__ void image_wait() {
 
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_imaged_kernel(attend_args a, attend_parts p) {
-    constexpr int PART = (int)image_part_bytes<HD, T>;
-    constexpr bool SCALED = wave_columns<HD, T>::SCALED;
-    __shared__ __attribute__((aligned(1024))) char sk[PART > IMAGE_WAVES * 4096 ? PART : IMAGE_WAVES * 4096]; /* (the queries pass through it) */
-    __shared__ __attribute__((aligned(1024))) char sv[PART];
+    constexpr int PART = image_part<HD, T>, ROOM = 2 * PART > IMAGE_WAVES * 4096 ? 2 * PART : IMAGE_WAVES * 4096; /* (the queries pass through the first) */
+    typedef wave_columns<HD, T, 32> columns;
+    /* arrays of their own: a copy into one is not waited for before the other is read */
+    __shared__ __attribute__((aligned(1024))) char even[ROOM];
+    __shared__ __attribute__((aligned(1024))) char odd[2 * PART];
     __shared__ attend_row srow[32 * IMAGE_WAVES];
     const int tid = threadIdx.x, split = blockIdx.y, h = blockIdx.x % a.n_kv, G = a.n_heads / a.n_kv, TR = 32 * IMAGE_WAVES / G;
     const int r0 = blockIdx.x / a.n_kv * TR, nr = min(TR, a.n - r0);
@@ -960,34 +997,51 @@ __global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_im
     lds_barrier();
     const group_span s = group_seen<true>(a, srow, 0, nr);
     const int4 at = p.meta[0];
-    /* seen, in chunks of 64 positions: c < n_sink, and from first on */
-    const int n_sink = (s.sink + 63) >> 6, first = max(n_sink, s.from >> 6), n_chunks = n_sink + max(((s.end + 63) >> 6) - first, 0);
-    const int per = (n_chunks + p.tile - 1) / p.tile, i0 = split * per, i1 = min(i0 + per, n_chunks);
-    wave_columns<HD, T> w;
-    w.template init<true>(a, srow, nr, sk, sv);
+    /* seen, in steps of 32 positions: u < n_sink, and from first on */
+    const int n_sink = (s.sink + 31) >> 5, first = max(n_sink, s.from >> 5), steps = n_sink + max(((s.end + 31) >> 5) - first, 0);
+    const int per = (steps + p.tile - 1) / p.tile, i0 = split * per, i1 = min(i0 + per, steps);
+    columns w;
+    w.template init<true>(a, srow, nr, even, even + PART);
     if (i0 < i1) {
-        w.load_queries(a, h, r0, nr, sk + (tid >> 6) * 4096);
-        const char* images = p.images + (size_t)h * p.slots * 2 * PART;
+        w.load_queries(a, h, r0, nr, even + (tid >> 6) * 4096);
+        const char* images = p.images + (size_t)h * p.slots * 4 * PART;
         const int4* meta = p.meta + 1 + (size_t)h * p.slots;
-        auto chunk = [&](int i) { return i < n_sink ? i : first + (i - n_sink); };
-        auto slot = [&](int i) { const int c = chunk(i); return c < at.x ? c : c - at.y; };
+        auto step = [&](int i) { return i < n_sink ? i : first + (i - n_sink); };
+        auto slot = [&](int i) { const int c = step(i) >> 1; return c < at.x ? c : c - at.y; };
+        auto image = [&](int i) { return images + ((size_t)slot(i) * 2 + (step(i) & 1)) * 2 * PART; };
         int e_run = 126;
-        lds_barrier(); /* every wave has its queries */
-        image_load<PART>(images + (size_t)slot(i0) * 2 * PART, sk);
-        for (int i = i0; i < i1; i++) {
-            const int4 m = meta[slot(i)];
-            image_wait(); /* the keys are there; every wave is past the last chunk's values */
-            image_load<PART>(images + ((size_t)slot(i) * 2 + 1) * PART, sv);
-            if (w.wave_on) {
-                w.scores();
-                if constexpr (SCALED) e_run = min(e_run, m.y);
-                const bool bad = (m.z | m.w) != 0;
-                w.weights(a, 64 * chunk(i), s.end, SCALED ? w.to_score * two_to(-m.x) : w.to_score, e_run, SCALED ? e_run - m.y : 0,
-                          bad ? reinterpret_cast<const uint32_t*>(&meta[slot(i)].z) : nullptr);
+        /* a step's powers and bad positions, by scalar loads (vector ones would wait for the copies asked for before them) */
+        auto meta_of = [&](int i) { return *(const __attribute__((address_space(4))) int4_*)(const int4_*)(meta + slot(i)); };
+        auto work = [&](int i, int4_ m, const char* room) {
+            const int u = step(i);
+            w.at(room, room + PART);
+            w.scores();
+            /* operands two steps ahead of their products */
+            constexpr int R = columns::PARTS ? 2 : 1, M = columns::PARTS ? 3 : 2;
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * R, 0);
+#pragma unroll
+            for (int g = 0; g < columns::KS - 2; g++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, M, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
             }
-            image_wait(); /* the values are there; every wave is past the keys */
-            if (i + 1 < i1) image_load<PART>(images + (size_t)slot(i + 1) * 2 * PART, sk);
-            if (w.wave_on) w.values();
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * M, 0);
+            if constexpr (columns::SCALED) e_run = min(e_run, m.y);
+            w.weights(a, 32 * u, s.end, columns::SCALED ? w.to_score * two_to(-m.x) : w.to_score, e_run, columns::SCALED ? e_run - m.y : 0,
+                      u & 1 ? m.w : m.z, 0);
+            w.values();
+        };
+        lds_barrier(); /* every wave has its queries */
+        image_load<2 * PART>(image(i0), even);
+        for (int i = i0; i < i1; i += 2) {
+            const int4_ m0 = meta_of(i);
+            image_wait(); /* this step's images are there; every wave is past the last one's */
+            if (i + 1 < i1) image_load<2 * PART>(image(i + 1), odd);
+            if (w.wave_on) work(i, m0, even);
+            if (i + 1 >= i1) break;
+            const int4_ m1 = meta_of(i + 1);
+            image_wait();
+            if (i + 2 < i1) image_load<2 * PART>(image(i + 2), even);
+            if (w.wave_on) work(i + 1, m1, odd);
         }
     }
     w.flush(a, p, split, h, r0);
