@@ -327,7 +327,7 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
 #define FEW_COLUMNS 32 /* a group with so many columns at most goes to few_part, any other to tile_part */
 
 template <int HD>
-constexpr int tile_waves = HD == 128 ? 8 : 4;
+constexpr int tile_waves = 4;
 /* Rows of a tile. Rows next to each other in a tile that read the same positions of the same sequence are a group. */
 template <int HD>
 __host__ __device__ constexpr int tile_rows(int G) { return 32 * tile_waves<HD> / G; }
@@ -839,7 +839,6 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
     w.template init<RUN>(a, srow, n_rows, sk, sv);
     if (c0 < c1) {
         if (tid < 2) sbad[tid] = 0;
-        w.load_queries(a, h, row0, n_rows, sk + (tid >> 6) * 4096);
         const T* ks = (const T*)a.k + (size_t)h * a.head_stride + (size_t)s.seq * a.seq_stride;
         const T* vs = (const T*)a.v + (size_t)h * a.head_stride + (size_t)s.seq * a.seq_stride;
         auto start = [&](int c) { return c < n_sink ? 64 * c : s.from + 64 * (c - n_sink); };
@@ -848,6 +847,7 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
         share rk, rv;
         rk.fetch(ks, a.pos_stride, start(c0), stop(c0));
         rv.fetch(vs, a.pos_stride, start(c0), stop(c0));
+        w.load_queries(a, h, row0, n_rows, sk + (tid >> 6) * 4096);
         rk.publish(smax);
         lds_barrier();
         for (int c = c0; c < c1; c++) {
@@ -1087,10 +1087,13 @@ __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(atten
     else own_part<HD, T, OWN_WAVES>(a, p, x % p.own, h, x / p.own, lds);
 }
 
+#define XCDS 8
 template <int HD, typename T, bool RUN>
-__global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_tile_kernel(attend_args a, attend_parts p) {
+__global__ __launch_bounds__(64 * tile_waves<HD>, HD == 128 ? 1 : 2) void attend_tile_kernel(attend_args a, attend_parts p) {
     __shared__ __attribute__((aligned(16))) char lds[tile_shape<HD, T, tile_waves<HD>>::LDS];
-    tile_part<HD, T, tile_waves<HD>, RUN>(a, p, blockIdx.y, blockIdx.x % a.n_kv, blockIdx.x / a.n_kv, lds);
+    /* the tiles of a head's split next to each other on one die, whose cache then serves all but the first */
+    const int tile = blockIdx.x / XCDS % p.tiles, pair = blockIdx.x / (XCDS * p.tiles) * XCDS + blockIdx.x % XCDS;
+    if (pair < a.n_kv * p.tile) tile_part<HD, T, tile_waves<HD>, RUN>(a, p, pair / a.n_kv, pair % a.n_kv, tile, lds);
 }
 
 /* HB heads of a row a block, SG threads for each four dimensions of one: the parts' factors once in LDS, then each
@@ -1182,7 +1185,7 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(attend_args a, attend
 /* How a call is cut into blocks. */
 static attend_parts plan(const attend_args& a) {
     attend_parts p = {};
-    const int G = a.n_heads / a.n_kv, nw = a.hd == 128 ? 8 : 4, rows = 32 * nw / G;
+    const int G = a.n_heads / a.n_kv, rows = (a.hd == 128 ? tile_rows<128>(G) : tile_rows<64>(G));
     p.tiles = (a.n + rows - 1) / rows;
     const long seen = a.window ? std::min<long>(a.own_max, (long)a.window + a.sinks) : a.own_max;
     const long blocks = 256; /* a block a compute unit */
@@ -1234,15 +1237,15 @@ size_t attend_work(const attend_args& a) {
 template <int HD, typename T>
 static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_t s) {
     constexpr int NW = tile_waves<HD>;
-    const unsigned heads = (unsigned)a.n_kv;
+    const unsigned heads = (unsigned)a.n_kv, tile_blocks = (heads * p.tile + XCDS - 1) / XCDS * XCDS * p.tiles;
     if (p.slots) {
         attend_image_kernel<HD, T><<<p.slots * heads, 256, 0, s>>>(a, p);
         attend_imaged_kernel<HD, T><<<dim3(p.tiles * heads, p.tile), 64 * IMAGE_WAVES, 0, s>>>(a, p);
     } else if (a.run) {
-        attend_tile_kernel<HD, T, true><<<dim3(p.tiles * heads, p.tile), 64 * NW, 0, s>>>(a, p);
+        attend_tile_kernel<HD, T, true><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else if (p.tile) {
         attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.tile + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
-        if (a.n * (a.n_heads / a.n_kv) > FEW_COLUMNS) attend_tile_kernel<HD, T, false><<<dim3(p.tiles * heads, p.tile), 64 * NW, 0, s>>>(a, p);
+        if (a.n * (a.n_heads / a.n_kv) > FEW_COLUMNS) attend_tile_kernel<HD, T, false><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else {
         attend_own_kernel<HD, T><<<dim3(a.n * heads, p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
     }
