@@ -326,11 +326,14 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
 
 #define FEW_COLUMNS 32 /* a group with so many columns at most goes to few_part, any other to tile_part */
 
+/* A tile: 32 columns each of TILE_COLUMNS waves; for tile_part of heads of 128 two waves take the same columns, each half of
+   a chunk's positions. */
+#define TILE_COLUMNS 4
 template <int HD>
-constexpr int tile_waves = 4;
+constexpr int tile_waves = HD == 128 ? 2 * TILE_COLUMNS : TILE_COLUMNS;
 /* Rows of a tile. Rows next to each other in a tile that read the same positions of the same sequence are a group. */
 template <int HD>
-__host__ __device__ constexpr int tile_rows(int G) { return 32 * tile_waves<HD> / G; }
+__host__ __device__ constexpr int tile_rows(int G) { return 32 * TILE_COLUMNS / G; }
 
 /* A tile's rows to LDS (the caller waits). */
 template <int NT>
@@ -465,10 +468,15 @@ struct tile_shape {
     static constexpr bool SCALED = !std::is_same<T, _Float16>::value;
     static constexpr int NT = 64 * NW, CC = HD / 4, U = 16 * CC / NT;    /* a thread's groups of 4 positions x 4 dimensions */
     static constexpr int HALF = 64 * HD;                                 /* values of one part of 64 positions' keys */
-    static constexpr int ROWS = 32 * NW;                                 /* the most rows of a tile */
-    static constexpr size_t HEAD = (2 * NW * 4 + 8 + 15) / 16 * 16, LDS = ROWS * sizeof(attend_row) + HEAD + (PARTS ? 4 : 2) * HALF * 2;
-    static_assert(NW * 4096 <= (PARTS ? 4 : 2) * HALF * 2, "the queries pass through the keys' and values' room");
-    static_assert(U >= 1 && U * NT == 16 * CC, "whole groups a thread");
+    static constexpr int ROWS = 32 * TILE_COLUMNS;                       /* the most rows of a tile */
+    static constexpr int SIDES = NW / TILE_COLUMNS, POS = 64 / SIDES;    /* waves of the same columns, each one's positions of a chunk */
+    static constexpr int KEYS = (PARTS ? 2 : 1) * HALF * 2;              /* bytes of a chunk's keys, and of its values */
+    static constexpr int SIDE = KEYS / SIDES;
+    static constexpr int MEET = SIDES > 1 ? TILE_COLUMNS * 64 * (HD / 2 + 8) * 4 : 0; /* what the sides exchange at the end */
+    static constexpr int ROOM = 2 * KEYS > MEET ? 2 * KEYS : MEET;
+    static constexpr size_t HEAD = (2 * NW * 4 + 8 + 15) / 16 * 16, LDS = ROWS * sizeof(attend_row) + HEAD + ROOM;
+    static_assert(NW * 4096 <= ROOM, "the queries pass through the keys' and values' room");
+    static_assert(SIDES * TILE_COLUMNS == NW && U >= 1 && U * NT == 16 * CC, "whole groups a thread");
 };
 
 /* Places in LDS (and in an image) of POS = 64 or 32 positions. Keys [part][POS][HD] in pieces of 8 dimensions, piece x of
@@ -611,7 +619,7 @@ struct wave_columns {
     }
     template <bool RUN>
     __device__ __forceinline__ void init(const attend_args& a, const attend_row* srow, int n_rows, const char* sk, const char* sv) {
-        const int lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv, col = 32 * (int)(threadIdx.x >> 6) + c32;
+        const int lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv, col = 32 * (int)(threadIdx.x / WAVE % TILE_COLUMNS) + c32;
         hh = lane >> 5;
         lr = col / G;
         g = col - lr * G;
@@ -634,9 +642,11 @@ struct wave_columns {
             for (int i = 0; i < 16; i++) O[d][i] = 0.0f;
     }
     /* The queries, through 4 KB of LDS of the wave's own, 32 dimensions at a time: loaded 128 bytes a column (a lane a
-       column would ask for 64 lines an instruction, 18000 cycles a block), taken as operand 16 s + 8 hh .. */
-    __device__ __forceinline__ void load_queries(const attend_args& a, int h, int row0, int n_rows, char* mine) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv;
+       column would ask for 64 lines an instruction, 18000 cycles a block), taken as operand 16 s + 8 hh ..; meanwhile asks
+       for more behind them */
+    template <typename F>
+    __device__ __forceinline__ void load_queries(const attend_args& a, int h, int row0, int n_rows, char* mine, F&& meanwhile) {
+        const int wave = threadIdx.x / WAVE % TILE_COLUMNS, lane = threadIdx.x & 63, c32 = lane & 31, G = a.n_heads / a.n_kv;
         float4 in[KS / 2][4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -645,6 +655,9 @@ struct wave_columns {
 #pragma unroll
             for (int t = 0; t < KS / 2; t++) in[t][i] = *reinterpret_cast<const float4*>(from + 32 * t);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        meanwhile();
+        __builtin_amdgcn_sched_barrier(0);
         /* a column's largest magnitude, from its eight lanes to its two */
         uint32_t mag = 0;
 #pragma unroll
@@ -795,6 +808,36 @@ struct wave_columns {
             }
         }
     }
+    /* Two waves of the same columns: half HALF of the dimensions of this one's O, m and l to room; the other's to this one's
+       O. m_run and e_out are the same in a column's two lanes. */
+    template <int HALF>
+    __device__ __forceinline__ void give(float4* room) const {
+        const int at = threadIdx.x % (WAVE * TILE_COLUMNS);
+#pragma unroll
+        for (int x = 0; x < DT * 2; x++) {
+            const f16v& o = O[HALF * DT / 2 + x / 4];
+            const int i = 4 * (x % 4);
+            room[x * WAVE * TILE_COLUMNS + at] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+        room[DT * 2 * WAVE * TILE_COLUMNS + at] = make_float4(m_run, l_run, 0.0f, 0.0f);
+    }
+    template <int HALF>
+    __device__ __forceinline__ void take(const float4* room) {
+        const int at = threadIdx.x % (WAVE * TILE_COLUMNS);
+        const float4 ml = room[DT * 2 * WAVE * TILE_COLUMNS + at];
+        const float m = fmaxf(m_run, ml.x), base = m == -INFINITY ? 0.0f : m, f = exp2_hw(m_run - base), g_ = exp2_hw(ml.x - base);
+        l_run = fmaf(l_run, f, ml.y * g_);
+        m_run = m;
+#pragma unroll
+        for (int x = 0; x < DT * 2; x++) {
+            const float4 y = room[x * WAVE * TILE_COLUMNS + at];
+            f16v& o = O[HALF * DT / 2 + x / 4];
+            const int i = 4 * (x % 4);
+            o[i] = fmaf(o[i], f, y.x * g_); o[i + 1] = fmaf(o[i + 1], f, y.y * g_); o[i + 2] = fmaf(o[i + 2], f, y.z * g_); o[i + 3] = fmaf(o[i + 3], f, y.w * g_);
+        }
+    }
+    /* dimensions 32 D0 .. 32 D1 - 1 */
+    template <int D0, int D1>
     __device__ __forceinline__ void flush(const attend_args& a, const attend_parts& p, int split, int h, int row0) {
         l_run += __shfl_xor(l_run, 32, WAVE);
         if (!there) return;
@@ -807,13 +850,13 @@ struct wave_columns {
             to = a.out + row * a.out_stride + (size_t)(h * G + g) * HD;
             f = l_run == 0.0f ? 0.0f : back / l_run;
         } else {
-            if (hh == 0) p.ml[part] = make_float2(m_run, l_run * two_to(-WEIGHT_EXP));
+            if (hh == 0 && D0 == 0) p.ml[part] = make_float2(m_run, l_run * two_to(-WEIGHT_EXP));
             if (l_run == 0.0f) return;
             to = p.acc + part * HD;
             f = back * two_to(-WEIGHT_EXP);
         }
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = D0; d < D1; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 *reinterpret_cast<float4*>(to + 32 * d + 8 * i + 4 * hh) = make_float4(O[d][4 * i] * f, O[d][4 * i + 1] * f, O[d][4 * i + 2] * f, O[d][4 * i + 3] * f);
@@ -827,16 +870,17 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
                                            const attend_row* srow, const group_span& s, char* lds) {
     typedef tile_shape<HD, T, NW> sh;
     typedef chunk_share<HD, T, 64 * NW> share;
-    const int tid = threadIdx.x;
+    typedef wave_columns<HD, T, sh::POS> columns;
+    const int tid = threadIdx.x, side = __builtin_amdgcn_readfirstlane(tid / (WAVE * TILE_COLUMNS));
     uint32_t* smax = reinterpret_cast<uint32_t*>(lds); /* [2][NW]: magnitudes of keys, of values */
     uint32_t* sbad = smax + 2 * NW;                    /* positions whose values are not finite */
     char* sk = lds + sh::HEAD;
-    char* sv = sk + (sh::PARTS ? 2 : 1) * sh::HALF * 2;
+    char* sv = sk + sh::KEYS;
     /* seen, in chunks of 64 */
     const int n_sink = (s.sink + 63) >> 6, n_chunks = n_sink + ((s.end - s.from + 63) >> 6);
     const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
-    wave_columns<HD, T, 64> w;
-    w.template init<RUN>(a, srow, n_rows, sk, sv);
+    columns w;
+    w.template init<RUN>(a, srow, n_rows, sk + side * sh::SIDE, sv + side * sh::SIDE);
     if (c0 < c1) {
         if (tid < 2) sbad[tid] = 0;
         const T* ks = (const T*)a.k + (size_t)h * a.head_stride + (size_t)s.seq * a.seq_stride;
@@ -845,9 +889,10 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
         auto stop = [&](int c) { return c < n_sink ? s.sink : s.end; };
         int e_run = 126; /* the values' power of two, the least so far */
         share rk, rv;
-        rk.fetch(ks, a.pos_stride, start(c0), stop(c0));
-        rv.fetch(vs, a.pos_stride, start(c0), stop(c0));
-        w.load_queries(a, h, row0, n_rows, sk + (tid >> 6) * 4096);
+        w.load_queries(a, h, row0, n_rows, sk + (tid >> 6) * 4096, [&] {
+            rk.fetch(ks, a.pos_stride, start(c0), stop(c0));
+            rv.fetch(vs, a.pos_stride, start(c0), stop(c0));
+        });
         rk.publish(smax);
         lds_barrier();
         for (int c = c0; c < c1; c++) {
@@ -861,7 +906,7 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
                 f = two_to(k);
                 from_keys *= two_to(-k);
             }
-            rk.store_keys(sk, f);
+            rk.template store_keys<sh::POS>(sk, f, sh::SIDE);
             rv.publish(smax + NW);
             if (c + 1 < c1) rk.fetch(ks, a.pos_stride, start(c + 1), stop(c + 1));
             lds_barrier();
@@ -874,9 +919,9 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
                 lds_barrier();
             }
             if constexpr (sh::SCALED) e_run = min(e_run, to_half_range(mag));
-            if (w.wave_on) w.weights(a, t0, t1, from_keys, e_run, 0, bad ? sbad[0] : 0, bad ? sbad[1] : 0);
+            if (w.wave_on) w.weights(a, t0 + side * sh::POS, t1, from_keys, e_run, 0, bad ? sbad[side] : 0, bad && sh::SIDES == 1 ? sbad[1] : 0);
             /* values to LDS; every wave is past the last chunk's values */
-            rv.store_values(sv, sh::SCALED ? two_to(e_run) : 1.0f);
+            rv.template store_values<sh::POS>(sv, sh::SCALED ? two_to(e_run) : 1.0f, sh::SIDE);
             if constexpr (sh::SCALED) {
                 if (c + 1 < c1) rk.publish(smax);
             }
@@ -886,7 +931,24 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
             if (w.wave_on) w.values();
         }
     }
-    w.flush(a, p, split, h, row0);
+    if constexpr (sh::SIDES == 1) {
+        w.template flush<0, columns::DT>(a, p, split, h, row0);
+    } else {
+        /* each side the other's half of what it has, through LDS, then to memory its own */
+        float4* room = reinterpret_cast<float4*>(sk);
+        float4* other = room + sh::MEET / 32;
+        lds_barrier(); /* every wave is past the last values */
+        if (side) w.template give<0>(other);
+        else w.template give<1>(room);
+        lds_barrier();
+        if (side) {
+            w.template take<1>(room);
+            w.template flush<columns::DT / 2, columns::DT>(a, p, split, h, row0);
+        } else {
+            w.template take<0>(other);
+            w.template flush<0, columns::DT / 2>(a, p, split, h, row0);
+        }
+    }
 }
 
 /* ---- a prompt's chunk over images of the cache ----
@@ -1003,7 +1065,7 @@ __global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_im
     columns w;
     w.template init<true>(a, srow, nr, even, even + PART);
     if (i0 < i1) {
-        w.load_queries(a, h, r0, nr, even + (tid >> 6) * 4096);
+        w.load_queries(a, h, r0, nr, even + (tid >> 6) * 4096, [] {});
         const char* images = p.images + (size_t)h * p.slots * 4 * PART;
         const int4* meta = p.meta + 1 + (size_t)h * p.slots;
         auto step = [&](int i) { return i < n_sink ? i : first + (i - n_sink); };
@@ -1044,7 +1106,7 @@ __global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_im
             if (w.wave_on) work(i + 1, m1, odd);
         }
     }
-    w.flush(a, p, split, h, r0);
+    w.template flush<0, columns::DT>(a, p, split, h, r0);
 }
 
 /* Split split of a tile's rows: RUN all together, otherwise its groups of many columns, one after another. */
@@ -1089,7 +1151,7 @@ __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(atten
 
 #define XCDS 8
 template <int HD, typename T, bool RUN>
-__global__ __launch_bounds__(64 * tile_waves<HD>, HD == 128 ? 1 : 2) void attend_tile_kernel(attend_args a, attend_parts p) {
+__global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_tile_kernel(attend_args a, attend_parts p) {
     __shared__ __attribute__((aligned(16))) char lds[tile_shape<HD, T, tile_waves<HD>>::LDS];
     /* the tiles of a head's split next to each other on one die, whose cache then serves all but the first */
     const int tile = blockIdx.x / XCDS % p.tiles, pair = blockIdx.x / (XCDS * p.tiles) * XCDS + blockIdx.x % XCDS;
