@@ -237,6 +237,27 @@ def test_rows_that_share(shape, window, sinks):
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_many_groups_in_a_tile(shape, window, sinks):
+    """More groups than a short prefix is cut into parts; several groups of many columns next to each other and between
+    those of few; a group that two tiles share."""
+    dtype, heads, kv, hd, layout = shape
+    G = heads // kv
+    with Device() as dev:
+        cache = Cache(dev, dtype, 11, 260, kv, hd, layout, seed=15)
+        many = -(-33 // G)  # rows of just more than 32 columns
+        sizes = [2] * 17 + [1, many, many, many + 1, 1, many, 3, 1, 1, 1, 2 * many, 1, many]
+        rows = []
+        for i, size in enumerate(sizes):
+            base, shared = (3 * i) % 11, (40 + i if i % 3 else 200 - 5 * i)
+            rows += [((base + 1 + j) % 11, min(259, shared + (7 * j) % 50), base, shared) for j in range(size)]
+        q = queries(len(rows), heads, hd, 16)
+        want, bound = cache.attend(q, rows, window, sinks)
+        for own_max, shared_max in ((60, 200), (260, 260), (60, 40)):
+            check(rows_call(dev, cache, q, rows, window, sinks, own_max, shared_max), want, bound, (own_max, shared_max))
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
 @pytest.mark.parametrize("n,pos0,window,sinks", [(1, 0, 0, 0), (1, 399, 33, 2), (2, 63, 1, 0), (37, 0, 0, 0), (37, 5, 20, 3), (130, 270, 64, 100),
                                                  (301, 99, 128, 1), (400, 0, 90, 4)])
 def test_runs(shape, n, pos0, window, sinks):

@@ -48,6 +48,7 @@ struct attend_parts {
     float* acc;  /* [n][n_kv][splits][G][hd]: its weighted values; unset where the sum is 0 */
     int own, tile; /* splits of the own parts and of the tiles' */
     int tiles;     /* tiles of rows */
+    int few_blocks, tile_blocks, busy; /* a tile's blocks, of a key-value head: of few_part, of tile_part, and of each those that get work */
     /* a run's chunks ready for LDS (attend_image_kernel): slots of them for each key-value head; 0: none */
     int slots;
     char* images;  /* [n_kv][slots] */
@@ -382,12 +383,27 @@ __device__ __forceinline__ group_span group_seen(const attend_args& a, const att
     return s;
 }
 
-/* The prefixes of a tile's groups of few columns. A unit is 16 columns of such a group; split x of the tile's p.tile takes
-   unit x mod (number of units), and of its positions part x / (number of units): one unit a block (as long as there are
-   splits enough), its part a long one. The other units' columns have nothing in split x. */
+/* How a tile's blocks take its units: block y takes unit y mod units, part y / units of its positions (there are blocks for
+   every unit). A unit's parts are the first of the tile's p.tile splits, the others get an empty part of its columns.
+   (Blocks that each took their part of unit after unit had 36 rows in groups of two behind 426 positions in 68 us; so 27.) */
+struct unit_share {
+    int units, y, parts;
+    __device__ __forceinline__ unit_share(int units_, int busy, int y_, int splits) : units(units_), y(y_), parts(min(max(busy / units_, 1), splits)) {}
+    __device__ __forceinline__ bool mine(int unit) const { return y % units == unit && y / units < parts; }
+    __device__ __forceinline__ int part() const { return y / units; }
+};
+/* The splits that a unit of n_cols columns from column col on leaves empty, of the part's share. */
+__device__ __forceinline__ void empty_parts(const attend_args& a, const attend_parts& p, const unit_share& u, int h, int row, int col, int n_cols) {
+    const int G = a.n_heads / a.n_kv, S = p.own + p.tile, c = col + (int)threadIdx.x;
+    if ((int)threadIdx.x >= n_cols) return;
+    for (int x = u.part() + u.parts; x < p.tile; x += u.parts)
+        p.ml[(((size_t)(row + c / G) * a.n_kv + h) * S + p.own + x) * G + c % G] = make_float2(-INFINITY, 0.0f);
+}
+
+/* Block y's of the prefixes of a tile's groups of few columns. A unit is 16 columns of such a group. */
 template <int HD, typename T, int NW>
-__device__ __forceinline__ void few_part(const attend_args& a, const attend_parts& p, int split, int h, int tile, char* lds) {
-    const int G = a.n_heads / a.n_kv, TR = tile_rows<HD>(G), r0 = tile * TR, nr = min(TR, a.n - r0), tid = threadIdx.x, S = p.own + p.tile;
+__device__ __forceinline__ void few_part(const attend_args& a, const attend_parts& p, int y, int h, int tile, char* lds) {
+    const int G = a.n_heads / a.n_kv, TR = tile_rows<HD>(G), r0 = tile * TR, nr = min(TR, a.n - r0);
     attend_row* srow = reinterpret_cast<attend_row*>(lds);
     char* rest = lds + tile_rows<HD>(1) * sizeof(attend_row);
     load_rows<64 * NW>(a, r0, nr, srow);
@@ -399,32 +415,25 @@ __device__ __forceinline__ void few_part(const attend_args& a, const attend_part
         if (n_cols <= FEW_COLUMNS) units += (n_cols + 15) >> 4;
     }
     if (!units) return;
-    const int parts = max(p.tile / units, 1); /* of a unit's positions */
+    const unit_share u(units, p.busy, y, p.tile);
     int unit = 0;
     for (int first = 0, next; first < nr; first = next) {
         next = group_end(srow, first, nr);
         const int n_cols = (next - first) * G;
         if (n_cols > FEW_COLUMNS) continue;
         for (int col = 0; col < n_cols; col += 16, unit++) {
+            if (!u.mine(unit)) continue;
             const int many = min(16, n_cols - col);
-            /* with more units than splits each split takes every p.tile-th */
-            const bool mine = units <= p.tile ? split % units == unit && split / units < parts : unit % p.tile == split;
-            if (!mine) {
-                if (tid < many) {
-                    const int c = col + tid;
-                    p.ml[(((size_t)(r0 + first + c / G) * a.n_kv + h) * S + p.own + split) * G + c % G] = make_float2(-INFINITY, 0.0f);
-                }
-                continue;
-            }
+            empty_parts(a, p, u, h, r0 + first, col, many);
             const group_span s = group_seen<false>(a, srow, first, next);
-            const int count = s.sink + (s.end - s.from), per = ((count + parts - 1) / parts + 15) & ~15;
+            const int count = s.sink + (s.end - s.from), per = ((count + u.parts - 1) / u.parts + 15) & ~15;
             positions at;
             at.begin = 0; at.n_sink = s.sink; at.from = s.from;
-            at.i0 = (int)min((long)(units <= p.tile ? split / units : 0) * per, (long)count);
+            at.i0 = (int)min((long)u.part() * per, (long)count);
             at.i1 = min(at.i0 + per, count);
             at.shared = INT32_MAX;
             at.other = at.mine = (size_t)s.seq * a.seq_stride;
-            columns_part<HD, T, NW, true>(a, p, at, p.own + split, h, r0 + first, srow + first, col, many, rest);
+            columns_part<HD, T, NW, true>(a, p, at, p.own + u.part(), h, r0 + first, srow + first, col, many, rest);
             lds_barrier();
         }
     }
@@ -863,10 +872,10 @@ struct wave_columns {
     }
 };
 
-/* Split split of what the columns of rows row0 + 0 .. n_rows - 1 see together: RUN, rows of one sequence, each up to itself;
+/* Split split of splits of what the columns of rows row0 + 0 .. n_rows - 1 see together: RUN, rows of one sequence, each up to itself;
    otherwise a group's shared prefix. srow are the rows. */
 template <int HD, typename T, int NW, bool RUN>
-__device__ __forceinline__ void group_part(const attend_args& a, const attend_parts& p, int split, int h, int row0, int n_rows,
+__device__ __forceinline__ void group_part(const attend_args& a, const attend_parts& p, int split, int splits, int h, int row0, int n_rows,
                                            const attend_row* srow, const group_span& s, char* lds) {
     typedef tile_shape<HD, T, NW> sh;
     typedef chunk_share<HD, T, 64 * NW> share;
@@ -878,7 +887,7 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
     char* sv = sk + sh::KEYS;
     /* seen, in chunks of 64 */
     const int n_sink = (s.sink + 63) >> 6, n_chunks = n_sink + ((s.end - s.from + 63) >> 6);
-    const int per = (n_chunks + p.tile - 1) / p.tile, c0 = split * per, c1 = min(c0 + per, n_chunks);
+    const int per = (n_chunks + splits - 1) / splits, c0 = split * per, c1 = min(c0 + per, n_chunks);
     columns w;
     w.template init<RUN>(a, srow, n_rows, sk + side * sh::SIDE, sv + side * sh::SIDE);
     if (c0 < c1) {
@@ -1109,21 +1118,30 @@ __global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_im
     w.template flush<0, columns::DT>(a, p, split, h, r0);
 }
 
-/* Split split of a tile's rows: RUN all together, otherwise its groups of many columns, one after another. */
+/* Block y's of a tile's rows: RUN its split of all together, otherwise of the groups of many columns, each a unit. */
 template <int HD, typename T, int NW, bool RUN>
-__device__ __forceinline__ void tile_part(const attend_args& a, const attend_parts& p, int split, int h, int tile, char* lds) {
+__device__ __forceinline__ void tile_part(const attend_args& a, const attend_parts& p, int y, int h, int tile, char* lds) {
     const int G = a.n_heads / a.n_kv, TR = tile_rows<HD>(G), r0 = tile * TR, nr = min(TR, a.n - r0);
     attend_row* srow = reinterpret_cast<attend_row*>(lds);
     char* rest = lds + tile_rows<HD>(1) * sizeof(attend_row);
     load_rows<64 * NW>(a, r0, nr, srow);
     lds_barrier();
     if constexpr (RUN) {
-        group_part<HD, T, NW, true>(a, p, split, h, r0, nr, srow, group_seen<true>(a, srow, 0, nr), rest);
+        group_part<HD, T, NW, true>(a, p, y, p.tile, h, r0, nr, srow, group_seen<true>(a, srow, 0, nr), rest);
     } else {
+        int units = 0;
         for (int first = 0, next; first < nr; first = next) {
             next = group_end(srow, first, nr);
-            if ((next - first) * G <= FEW_COLUMNS) continue;
-            group_part<HD, T, NW, false>(a, p, split, h, r0 + first, next - first, srow + first, group_seen<false>(a, srow, first, next), rest);
+            units += (next - first) * G > FEW_COLUMNS;
+        }
+        if (!units) return;
+        const unit_share u(units, p.busy, y, p.tile);
+        int unit = 0;
+        for (int first = 0, next; first < nr; first = next) {
+            next = group_end(srow, first, nr);
+            if ((next - first) * G <= FEW_COLUMNS || !u.mine(unit++)) continue;
+            empty_parts(a, p, u, h, r0 + first, 0, (next - first) * G);
+            group_part<HD, T, NW, false>(a, p, u.part(), u.parts, h, r0 + first, next - first, srow + first, group_seen<false>(a, srow, first, next), rest);
             lds_barrier();
         }
     }
@@ -1140,13 +1158,19 @@ __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_own_kernel(attend_ar
     own_part<HD, T, OWN_WAVES>(a, p, blockIdx.y, blockIdx.x % a.n_kv, blockIdx.x / a.n_kv, lds);
 }
 
-/* The prefixes of groups of few columns, tile by tile, then the rows' own parts. */
+/* The prefixes of groups of few columns and the rows' own parts. */
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(attend_args a, attend_parts p) {
     __shared__ __attribute__((aligned(16))) char lds[columns_lds<HD, OWN_WAVES> + tile_rows<HD>(1) * sizeof(attend_row)];
-    const int tiles = p.tiles * a.n_kv * p.tile, b = (int)blockIdx.x < tiles ? blockIdx.x : blockIdx.x - tiles, h = b % a.n_kv, x = b / a.n_kv;
-    if ((int)blockIdx.x < tiles) few_part<HD, T, OWN_WAVES>(a, p, x % p.tile, h, x / p.tile, lds);
-    else own_part<HD, T, OWN_WAVES>(a, p, x % p.own, h, x / p.own, lds);
+    /* first the blocks of few_part that get work if any do, behind the own parts those that only many groups need (idle ones
+       before the own parts: 40 rows in groups of eight behind 2048 positions 61.5 us; so 53.9) */
+    const int heads = a.n_kv, h = blockIdx.x % heads, busy = min(p.busy, p.few_blocks) * p.tiles, own = a.n * p.own, b = blockIdx.x / heads;
+    if (b >= busy && b < busy + own) {
+        own_part<HD, T, OWN_WAVES>(a, p, (b - busy) % p.own, h, (b - busy) / p.own, lds);
+    } else {
+        const int x = b < busy ? b : b - own; /* block x / tiles of tile x mod tiles */
+        few_part<HD, T, OWN_WAVES>(a, p, x / p.tiles, h, x % p.tiles, lds);
+    }
 }
 
 #define XCDS 8
@@ -1155,7 +1179,7 @@ __global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_tile_kernel(att
     __shared__ __attribute__((aligned(16))) char lds[tile_shape<HD, T, tile_waves<HD>>::LDS];
     /* the tiles of a head's split next to each other on one die, whose cache then serves all but the first */
     const int tile = blockIdx.x / XCDS % p.tiles, pair = blockIdx.x / (XCDS * p.tiles) * XCDS + blockIdx.x % XCDS;
-    if (pair < a.n_kv * p.tile) tile_part<HD, T, tile_waves<HD>, RUN>(a, p, pair / a.n_kv, pair % a.n_kv, tile, lds);
+    if (pair < a.n_kv * p.tile_blocks) tile_part<HD, T, tile_waves<HD>, RUN>(a, p, pair / a.n_kv, pair % a.n_kv, tile, lds);
 }
 
 /* HB heads of a row a block, SG threads for each four dimensions of one: the parts' factors once in LDS, then each
@@ -1265,14 +1289,20 @@ static attend_parts plan(const attend_args& a) {
             return p;
         }
         const long chunks = (a.window ? std::min<long>(a.own_max, (long)a.window + a.sinks + rows) : a.own_max) / 64 + 1;
-        p.tile = (int)std::min<long>(std::min<long>(chunks, 64), std::max<long>(1, blocks / ((long)p.tiles * a.n_kv)));
+        p.tile = p.tile_blocks = (int)std::min<long>(std::min<long>(chunks, 64), std::max<long>(1, blocks / ((long)p.tiles * a.n_kv)));
         return p;
     }
     if (a.shared_max) {
-        /* only groups of few columns: two of their blocks a compute unit */
+        /* of groups of few columns two blocks a compute unit, of others one; a tile's groups may need a block each */
         const long chunks = (a.window ? std::min<long>(a.shared_max, (long)a.window + a.sinks) : a.shared_max) / 64 + 1;
         const bool few = a.n * G <= FEW_COLUMNS;
-        p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), std::max<long>(1, (few ? 2 : 1) * blocks / ((long)p.tiles * a.n_kv)));
+        /* (with twice as many splits the same 40 rows took 65 us for 53, and 32 rows behind 8192 positions 60 for 45) */
+        const long at_once = std::max<long>(1, blocks / ((long)p.tiles * a.n_kv));
+        const long groups = std::min(a.n, rows), big = std::min<long>(32 * TILE_COLUMNS / (FEW_COLUMNS + 1), groups); /* a tile's units at most: a row is one at most */
+        p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), few ? 2 * at_once : at_once);
+        p.busy = few ? p.tile : (int)at_once;
+        p.few_blocks = (int)std::min<long>(std::max<long>(p.busy, groups), groups * p.tile);
+        p.tile_blocks = (int)std::min<long>(std::max<long>(p.busy, big), big * p.tile);
     }
     p.own = (int)std::min<long>(std::min<long>((seen + 16 * OWN_WAVES - 1) / (16 * OWN_WAVES), ATTEND_SPLITS_MAX), std::max<long>(1, 1024 / ((long)a.n * a.n_kv)));
     if (a.splits) p.own = std::min(a.splits, ATTEND_SPLITS_MAX);
@@ -1299,14 +1329,14 @@ size_t attend_work(const attend_args& a) {
 template <int HD, typename T>
 static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_t s) {
     constexpr int NW = tile_waves<HD>;
-    const unsigned heads = (unsigned)a.n_kv, tile_blocks = (heads * p.tile + XCDS - 1) / XCDS * XCDS * p.tiles;
+    const unsigned heads = (unsigned)a.n_kv, tile_blocks = (heads * p.tile_blocks + XCDS - 1) / XCDS * XCDS * p.tiles;
     if (p.slots) {
         attend_image_kernel<HD, T><<<p.slots * heads, 256, 0, s>>>(a, p);
         attend_imaged_kernel<HD, T><<<dim3(p.tiles * heads, p.tile), 64 * IMAGE_WAVES, 0, s>>>(a, p);
     } else if (a.run) {
         attend_tile_kernel<HD, T, true><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else if (p.tile) {
-        attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.tile + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
+        attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.few_blocks + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
         if (a.n * (a.n_heads / a.n_kv) > FEW_COLUMNS) attend_tile_kernel<HD, T, false><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else {
         attend_own_kernel<HD, T><<<dim3(a.n * heads, p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
