@@ -8,11 +8,13 @@
  * with a running maximum and sum, both and the weighted values in float32 (the scores in units of log 2, so that
  * exp is exp2). Two kinds of block take parts of it:
  *
- *   columns_part  up to 32 columns (row, query head) of one key-value head: a row's own positions, or a prefix that a few
- *                 rows share. Each wave takes other positions, straight to registers. Bound by the cache's bytes;
- *                 products on v_mfma_f32_16x16x4_f32.
- *   tile_part     positions that many columns see (a shared prefix, a prompt's chunk): 32 columns a wave, 64 positions at a
- *                 time through LDS, read once for all the block's columns. Products on v_mfma_f32_32x32x16_f16.
+ *   columns_part  16 columns (row, query head) of one key-value head: a row's own positions, or a prefix that few columns
+ *                 share. Each wave takes other positions, straight to registers. Bound by the cache's bytes; products on
+ *                 v_mfma_f32_16x16x4_f32.
+ *   group_part    positions that many columns see (a shared prefix, a prompt's chunk): 32 columns a wave, 128 a block, 64
+ *                 positions at a time through LDS, read once for all the block's columns. Products on
+ *                 v_mfma_f32_32x32x16_f16. A long chunk of a prompt takes the same steps from images of the cache
+ *                 (attend_image_kernel, attend_imaged_kernel).
  *
  * Where a row's positions are split over several blocks, each leaves its maximum, sum and weighted values, and
  * attend_merge_kernel joins them.
@@ -48,6 +50,7 @@ struct attend_parts {
     float* acc;  /* [n][n_kv][splits][G][hd]: its weighted values; unset where the sum is 0 */
     int own, tile; /* splits of the own parts and of the tiles' */
     int tiles;     /* tiles of rows */
+    int few;       /* a group's columns for few_part at most */
     int few_blocks, tile_blocks, busy; /* a tile's blocks, of a key-value head: of few_part, of tile_part, and of each those that get work */
     /* a run's chunks ready for LDS (attend_image_kernel): slots of them for each key-value head; 0: none */
     int slots;
@@ -325,7 +328,12 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
 
 /* ---- rows that share ---- */
 
-#define FEW_COLUMNS 32 /* a group with so many columns at most goes to few_part, any other to tile_part */
+/* A group with so many columns at most goes to few_part, any other to tile_part; a call of FEW_CALL columns or fewer has no
+   other groups. 8 rows of 8 heads a key-value head behind 777 positions (float32): 18 us in few_part, 25 in tile_part;
+   behind 4096, 24 and 31. Four such groups, 32 rows: behind 777 25 and 30, behind 4096 49 and 43 (bfloat16 54 and 34). Eight
+   groups of 32 columns behind 4096: 51 and 55 (bfloat16 55 and 43). */
+#define FEW_COLUMNS 32
+#define FEW_CALL 64
 
 /* A tile: 32 columns each of TILE_COLUMNS waves; for tile_part of heads of 128 two waves take the same columns, each half of
    a chunk's positions. */
@@ -412,7 +420,7 @@ __device__ __forceinline__ void few_part(const attend_args& a, const attend_part
     for (int first = 0, next; first < nr; first = next) {
         next = group_end(srow, first, nr);
         const int n_cols = (next - first) * G;
-        if (n_cols <= FEW_COLUMNS) units += (n_cols + 15) >> 4;
+        if (n_cols <= p.few) units += (n_cols + 15) >> 4;
     }
     if (!units) return;
     const unit_share u(units, p.busy, y, p.tile);
@@ -420,7 +428,7 @@ __device__ __forceinline__ void few_part(const attend_args& a, const attend_part
     for (int first = 0, next; first < nr; first = next) {
         next = group_end(srow, first, nr);
         const int n_cols = (next - first) * G;
-        if (n_cols > FEW_COLUMNS) continue;
+        if (n_cols > p.few) continue;
         for (int col = 0; col < n_cols; col += 16, unit++) {
             if (!u.mine(unit)) continue;
             const int many = min(16, n_cols - col);
@@ -978,7 +986,8 @@ __device__ __forceinline__ int2 image_slots(const attend_args& a, uint32_t far, 
     return make_int2(n_sink, max(n_sink, from >> 6) - n_sink);
 }
 
-/* Block (key-value head, slot): 64 positions. */
+/* Block (key-value head, slot): 64 positions. Bound by bytes: the 5120 positions behind 1024 rows of a 4096 window, 21 MB in
+   and as many out in 10-11 us. */
 template <int HD, typename T>
 __global__ __launch_bounds__(256) void attend_image_kernel(attend_args a, attend_parts p) {
     typedef chunk_share<HD, T, 256> share;
@@ -1054,6 +1063,10 @@ __device__ __forceinline__ void image_wait() {
     lds_barrier();
 }
 
+/* Block (tile, key-value head), split. Bound by the matrix cores and what the waves do beside them: 1024 rows of 32 heads with
+   a 4096 window and four sinks (4 heads of 128, float32), 206 GFLOP as three products each, in 185-205 us: 1.0-1.1 PFLOP/s
+   of the 2.07 that products alone reach; 57 % of a SIMD's cycles are products, 25 % of a wave's waits for the others of its
+   block. (The next step's scores formed beside this one's weights, 256 registers: 229 us for the call, 214 so.) */
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * IMAGE_WAVES, HD == 128 ? 2 : 3) void attend_imaged_kernel(attend_args a, attend_parts p) {
     constexpr int PART = image_part<HD, T>, ROOM = 2 * PART > IMAGE_WAVES * 4096 ? 2 * PART : IMAGE_WAVES * 4096; /* (the queries pass through the first) */
@@ -1132,14 +1145,14 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
         int units = 0;
         for (int first = 0, next; first < nr; first = next) {
             next = group_end(srow, first, nr);
-            units += (next - first) * G > FEW_COLUMNS;
+            units += (next - first) * G > p.few;
         }
         if (!units) return;
         const unit_share u(units, p.busy, y, p.tile);
         int unit = 0;
         for (int first = 0, next; first < nr; first = next) {
             next = group_end(srow, first, nr);
-            if ((next - first) * G <= FEW_COLUMNS || !u.mine(unit++)) continue;
+            if ((next - first) * G <= p.few || !u.mine(unit++)) continue;
             empty_parts(a, p, u, h, r0 + first, 0, (next - first) * G);
             group_part<HD, T, NW, false>(a, p, u.part(), u.parts, h, r0 + first, next - first, srow + first, group_seen<false>(a, srow, first, next), rest);
             lds_barrier();
@@ -1151,14 +1164,18 @@ __device__ __forceinline__ void tile_part(const attend_args& a, const attend_par
 
 #define OWN_WAVES 4
 
-/* Rows' own parts alone: block (row, key-value head), split. */
+/* Rows' own parts alone: block (row, key-value head), split. Bound by the cache's bytes: 32 rows of a 4096 window and four
+   sinks (f16, 4 heads of 128), 270 MB in 69-71 us, 3.8-3.9 TB/s, where a large copy reaches 4.8. One row's 1028 float32
+   positions: 7 us, five of them a launch, the rows and two dependent steps. */
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_own_kernel(attend_args a, attend_parts p) {
     __shared__ __attribute__((aligned(16))) char lds[columns_lds<HD, OWN_WAVES>];
     own_part<HD, T, OWN_WAVES>(a, p, blockIdx.y, blockIdx.x % a.n_kv, blockIdx.x / a.n_kv, lds);
 }
 
-/* The prefixes of groups of few columns and the rows' own parts. */
+/* The prefixes of groups of few columns and the rows' own parts. 40 rows of 16 heads of 128 in groups of eight behind 2048
+   positions (bfloat16): 139 MB in 46-48 us, 3 TB/s; the blocks of a group's prefix are long ones, and its products (16
+   columns, half of them used) run beside the loads of the next step. 32 rows' own 256 positions (float32): 11 us. */
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(attend_args a, attend_parts p) {
     __shared__ __attribute__((aligned(16))) char lds[columns_lds<HD, OWN_WAVES> + tile_rows<HD>(1) * sizeof(attend_row)];
@@ -1173,6 +1190,10 @@ __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(atten
     }
 }
 
+/* 32 rows of 32 heads behind 8192 positions (4 heads of 128, float32): 32 us, of which a block works 27: 2 for its rows, 6
+   until its queries and first chunk are there, 15 for four chunks (7700 cycles each, 3100 of them products) and 4 to
+   exchange and write. Blocks of 256 columns and half as many chunks wrote and read back twice as many parts (the call 54
+   us for 45). */
 #define XCDS 8
 template <int HD, typename T, bool RUN>
 __global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_tile_kernel(attend_args a, attend_parts p) {
@@ -1183,7 +1204,8 @@ __global__ __launch_bounds__(64 * tile_waves<HD>, 2) void attend_tile_kernel(att
 }
 
 /* HB heads of a row a block, SG threads for each four dimensions of one: the parts' factors once in LDS, then each
-   thread adds up every SG-th part, all its loads asked for before the first is used. */
+   thread adds up every SG-th part, all its loads asked for before the first is used. Bound by the parts'
+   bytes: 1024 rows of 32 heads in two parts, 50 MB in 12 us, 4.3 TB/s; 32 rows in 40 parts, 21 MB in 5.5. */
 #define MERGE_SPLITS 512 /* parts of a row at most */
 #define MERGE_AHEAD 8
 template <int HD, int SG>
@@ -1264,8 +1286,10 @@ __global__ __launch_bounds__(256) void attend_merge_kernel(attend_args a, attend
     if (head < a.n_heads) reinterpret_cast<float4*>(a.out + (size_t)row * a.out_stride + (size_t)head * HD)[d] = o;
 }
 
-/* A run of so many tiles or more goes over images, if they take no more bytes than this. */
-#define IMAGE_TILES 8
+/* A run of so many tiles or more goes over images, if they take no more bytes than this. Behind 3000 positions, 32 heads of
+   128 on 4, float32: 8 tiles 46 us over images and 41 without, 12 tiles 56 and 81, 21 tiles 79 and 135; 8 heads of 64 on 2,
+   bfloat16: 6 tiles 25 and 18, 11 tiles 28 and 29. */
+#define IMAGE_TILES 9
 #define IMAGE_BYTES_MAX ((size_t)256 << 20)
 
 /* How a call is cut into blocks. */
@@ -1295,7 +1319,8 @@ static attend_parts plan(const attend_args& a) {
     if (a.shared_max) {
         /* of groups of few columns two blocks a compute unit, of others one; a tile's groups may need a block each */
         const long chunks = (a.window ? std::min<long>(a.shared_max, (long)a.window + a.sinks) : a.shared_max) / 64 + 1;
-        const bool few = a.n * G <= FEW_COLUMNS;
+        const bool few = (long)a.n * G <= FEW_CALL;
+        p.few = few ? FEW_CALL : FEW_COLUMNS;
         /* (with twice as many splits the same 40 rows took 65 us for 53, and 32 rows behind 8192 positions 60 for 45) */
         const long at_once = std::max<long>(1, blocks / ((long)p.tiles * a.n_kv));
         const long groups = std::min(a.n, rows), big = std::min<long>(32 * TILE_COLUMNS / (FEW_COLUMNS + 1), groups); /* a tile's units at most: a row is one at most */
@@ -1337,7 +1362,7 @@ static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_
         attend_tile_kernel<HD, T, true><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else if (p.tile) {
         attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.few_blocks + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
-        if (a.n * (a.n_heads / a.n_kv) > FEW_COLUMNS) attend_tile_kernel<HD, T, false><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
+        if ((long)a.n * (a.n_heads / a.n_kv) > p.few) attend_tile_kernel<HD, T, false><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else {
         attend_own_kernel<HD, T><<<dim3(a.n * heads, p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
     }
