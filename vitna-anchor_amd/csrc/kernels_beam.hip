@@ -56,6 +56,8 @@ static __host__ __device__ size_t beam_sums_bytes(size_t slices) { return (slice
 /* x at i comes before y at j: larger, or equal and of lower index */
 __device__ __forceinline__ bool beam_before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
+/* Bound by the logits' bytes where they are many: 64 rows of 151936, 39 MB in 14-16 us, 2.4-2.8 TB/s; by the chain of its
+   steps where they are few (4 rows: 7 us). */
 template <int E, bool VEC>
 __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_args a, int splits) {
     __shared__ float sm[BEAM_WAVES], ss[BEAM_WAVES];
@@ -267,8 +269,10 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
 #define PICK_HELD 7168 /* candidates that are kept in LDS */
 #define PICK_BINS 2048
 #define PICK_CAP 512   /* continuations that are ranked by counting, at most */
-#define PICK_FEW 96    /* and without cutting them first */
+#define PICK_FEW 96    /* and without cutting them first (with 512: 8 beams of 16 kept 24 us for 21, 8 groups of those 26 for 23; with 32: 15 for 13 where 8 are kept) */
 
+/* Latency: a block a group, its slices' sums and candidates (one load each), the bound, the candidates that reach it, their
+   ranks. 9 us for 4 or 8 beams of 151936, 15 for 32 beams of 40000 with 64 kept. */
 __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_args a, int splits) {
     __shared__ beam_cand s_cand[PICK_HELD];
     __shared__ double s_score[64], s_log[64]; /* of a beam: its score (-inf: it has no continuations), log of its sum of exponentials */
@@ -495,25 +499,28 @@ __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_arg
     none_from(keep);
 }
 
-/* Values a lane of the scan: 64 where that leaves most compute units a block, or where slices of 16 would leave more
-   candidates than the pick holds in LDS; else 16. */
-static int beam_lane_values(int rows, int width, size_t vocab, int keep) {
+/* Values a lane of the scan: 64 where that leaves most compute units a block, or where slices of 16 would be so many a group
+   that the pick of their candidates costs more than the scan gains (112 of 64 are what it holds in LDS); else 16. In us of a
+   call, 16 and 64 (groups x width, vocabulary, keep): 1 x 2, 151936, 4: 11.6, 13.8; 1 x 4, 151936, 8 (152 slices): 15.9, 14.9;
+   1 x 8, 151936, 16: 20.6, 18.5; 1 x 8, 32000, 16 (64 slices): 15.8, 16.3; 16 x 4, 32000, 8: 13.6, 15.4; 32 x 4, 32000, 8:
+   16.0, 15.5; 8 x 8, 151936, 16: 36, 23. */
+static int beam_lane_values(int rows, int width, size_t vocab) {
     const size_t small = (vocab + BEAM_WAVES * 64 * 16 - 1) / (BEAM_WAVES * 64 * 16);
-    return (size_t)rows * vocab >= (size_t)224 * BEAM_WAVES * 64 * 64 || width * small * keep > PICK_HELD ? 64 : 16;
+    return (size_t)rows * vocab >= (size_t)224 * BEAM_WAVES * 64 * 64 || (size_t)width * small * 64 > PICK_HELD ? 64 : 16;
 }
-static int beam_splits(int rows, int width, size_t vocab, int keep) {
-    const size_t slice = (size_t)BEAM_WAVES * 64 * beam_lane_values(rows, width, vocab, keep);
+static int beam_splits(int rows, int width, size_t vocab) {
+    const size_t slice = (size_t)BEAM_WAVES * 64 * beam_lane_values(rows, width, vocab);
     return (int)((vocab + slice - 1) / slice);
 }
 
 size_t beam_select_work(int groups, int width, size_t vocab, int keep) {
-    const size_t slices = (size_t)groups * width * beam_splits(groups * width, width, vocab, keep);
+    const size_t slices = (size_t)groups * width * beam_splits(groups * width, width, vocab);
     return beam_sums_bytes(slices) + slices * keep * sizeof(beam_cand);
 }
 
 hipError_t launch_beam_select(const beam_select_args& a, hipStream_t s) {
     if (a.groups < 1 || a.width < 1 || a.width > 64 || a.keep < 1 || a.keep > 64) return hipErrorInvalidValue;
-    const int rows = a.groups * a.width, splits = beam_splits(rows, a.width, a.vocab, a.keep), E = beam_lane_values(rows, a.width, a.vocab, a.keep);
+    const int rows = a.groups * a.width, splits = beam_splits(rows, a.width, a.vocab), E = beam_lane_values(rows, a.width, a.vocab);
     if ((size_t)rows * splits > ((size_t)1 << 23)) return hipErrorInvalidValue; /* threads of a launch stay within 32 bits */
     const int grid = rows * splits;
     const bool vec = ((uintptr_t)a.logits & 15) == 0 && a.stride % 4 == 0;
@@ -532,15 +539,13 @@ hipError_t launch_beam_select(const beam_select_args& a, hipStream_t s) {
    A thread takes the same few bytes of every beam of a group: all that moves is read before any is written, so a beam
    may take another's place while that takes a third's, and no thread waits for another. What it takes lies at the same
    place in every layer, so a block walks over layers with its beams and offsets at hand. Bound by memory: half a beam's
-   worth is read and half written for each that changes. */
+   worth is read and half written for each that changes (8 groups of 8 beams over 24 layers, 830 MB in 160-180 us, 4.6-5.2
+   TB/s). */
 
-/* the bytes a thread takes of a beam: what W of them leave room for in registers */
-template <int W>
-using reorder_piece = std::conditional_t<W <= 32, u32x4, uint2>;
+typedef u32x4 piece_t; /* what a thread takes of a beam, of 64 beams too (400 registers; pieces of 8 bytes: 33 beams 28 us for 17, 64 beams 36 for 29) */
 
 template <int W>
 __global__ __launch_bounds__(256) void kv_reorder_kernel(kv_reorder_args a) {
-    typedef reorder_piece<W> piece_t;
     __shared__ int s_from[W], s_to[W];
     const int group = blockIdx.z, tid = threadIdx.x;
     if (tid < W) {
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(kv_reorder_args a) {
 template <int W>
 static void reorder(const kv_reorder_args& a, hipStream_t s) {
     /* blocks over the positions, then over the layers until there are eight a compute unit */
-    const int64_t pieces = (int64_t)a.longest * a.n_kv * (int64_t)(a.dim_bytes / sizeof(reorder_piece<W>));
+    const int64_t pieces = (int64_t)a.longest * a.n_kv * (int64_t)(a.dim_bytes / sizeof(piece_t));
     const unsigned x = (unsigned)std::min<int64_t>(std::max<int64_t>((pieces + 255) / 256, 1), 4096);
     const int64_t want = 2048 / ((int64_t)x * a.groups) + 1;
     kv_reorder_kernel<W><<<dim3(x, (unsigned)std::min<int64_t>(2 * a.layers, want), a.groups), 256, 0, s>>>(a);
