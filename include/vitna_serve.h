@@ -72,7 +72,11 @@ size_t vitna_hip_attention_rows_work(const vitna_hip_kv_view_t* c, size_t n, siz
     the most that rows share (0: read them with the row's own); they size the
     launch, and rows beyond them get the same values, later. The keys and
     values of the positions that a row sees have to be in the cache; what lies
-    at the others, NaN among it, has no effect on the row. */
+    at the others, infinities and NaN among it, has no effect on the row, but
+    for this: where many rows see positions together, their keys and their
+    values are taken to within 2^-20 of themselves and 2^-28 of the largest
+    finite one of the positions before and around them that any of the rows
+    sees. */
 bool vitna_hip_attention_rows(const vitna_hip_kv_view_t* c, const float* q, size_t q_stride, const vitna_hip_attention_row_t* rows, size_t n,
                               size_t own_max, size_t shared_max, float* out, size_t out_stride, void* work, size_t work_bytes, void* stream,
                               char* err, size_t err_len);

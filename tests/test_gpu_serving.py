@@ -345,6 +345,36 @@ def test_what_a_row_does_not_see_does_not_matter(dtype, bad):
                 assert sees[i] == (not np.isfinite(out[i]).all()), rows[i]
 
 
+@pytest.mark.parametrize("dtype,hd,huge", [("f32", 128, 1e30), ("f32", 64, -3e38), ("bf16", 128, -3e38), ("bf16", 64, 1e30), ("f16", 128, 65504.0)])
+@pytest.mark.parametrize("window,sinks", [(70, 5), (70, 0), (3, 64), (64, 70), (200, 1)])
+def test_large_numbers_that_no_row_sees(dtype, hd, huge, window, sinks):
+    """Numbers of the type's largest size where no row looks: before the first row's window, behind the last row, in the
+    pieces that a block reads of either side; a query of them leaves the other rows as they are."""
+    heads, kv, ctx = 16, 2, 600
+    r = np.random.RandomState(21)
+    k, v = r.standard_normal((2, ctx, kv, hd)), r.standard_normal((2, ctx, kv, hd))
+    with Device() as dev:
+        clean = Cache(dev, dtype, 2, ctx, kv, hd, k=k.copy(), v=v.copy())
+        for pos0, n in ((303, 200), (257, 20), (64, 130)):
+            seen = np.zeros(ctx, bool)
+            for p in (pos0, pos0 + n - 1):
+                seen[visible(p, window, sinks)] = True
+            seen[pos0:pos0 + n] = True
+            dirty_k, dirty_v = k.copy(), v.copy()
+            dirty_k[:, ~seen], dirty_v[:, ~seen] = huge, huge
+            cache = Cache(dev, dtype, 2, ctx, kv, hd, k=dirty_k, v=dirty_v)
+            q = queries(n, heads, hd, 22)
+            some = sorted({0, 1, n // 2, n - 2, n - 1})
+            want, bound = clean.attend(q[some], [(1, pos0 + i, 0, 0) for i in some], window, sinks)
+            q[3] = np.float32(1e30)
+            q[5] = np.nan
+            check(run_call(dev, cache, q, 1, pos0, window, sinks)[some], want, bound, ("run", pos0, n))
+            rows = [(0, pos0 + i, 1, pos0 + 1) for i in range(min(n, 40))]
+            q = queries(len(rows), heads, hd, 23)
+            want, bound = clean.attend(q, rows, window, sinks)
+            check(rows_call(dev, cache, q, rows, window, sinks, 100, 600), want, bound, ("rows", pos0, n))
+
+
 def test_wide_scores_and_a_scale():
     """Scores of thousands: one position takes all the weight; and scores all alike, far below zero."""
     with Device() as dev:

@@ -66,6 +66,8 @@ def test_attention_arguments_refused():
     refused(lambda: va.attention_rows(v, AT + 4, AT, 5, AT, AT, work), "aligned")
     refused(lambda: va.attention_rows(v, AT, AT + 4, 5, AT, AT, work), "aligned")
     refused(lambda: va.attention_rows(v, AT, AT, 5, AT, AT, work, out_stride=1020), "floats apart")
+    refused(lambda: va.attention_rows(v, AT, AT, 5, AT, AT, work, out_stride=1028), "out is q")
+    refused(lambda: va.attention_run(v, 0, 0, AT, 5, AT, AT, 1 << 20, q_stride=2048), "out is q")
     refused(lambda: va.attention_rows(v, AT, AT, 5, AT, AT, work, q_stride=1025), "floats apart")
     refused(lambda: va.attention_rows(v, AT, AT, 5, AT, AT, work), "not device memory")
     refused(lambda: va.attention_rows(view(k=None), AT, AT, 5, AT, AT, work), "k is missing")

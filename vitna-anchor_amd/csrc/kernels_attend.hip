@@ -519,16 +519,21 @@ template <int HD, typename T, int NT>
 struct chunk_share {
     static constexpr int CC = HD / 4, U = 16 * CC / NT;
     vec<T, 4> x[U][4];
-    /* positions t0 .. t1 - 1 (64 at most) of src (a head's positions); those behind t1 read the last again: their scores are masked */
-    __device__ __forceinline__ void fetch(const T* src, size_t pos_stride, int t0, int t1) {
-        const uint32_t most = (uint32_t)(min(t1 - t0, 64) - 1), pos_bytes = (uint32_t)(pos_stride * sizeof(T)); /* 64 of them stay within 31 bits */
+    /* positions t0 .. t1 - 1 (64 at most) of src (a head's positions). Those that no row sees, behind t1 and gap0 .. gap1 - 1, take
+       a place that one does (their scores are masked, and their values would set the others' powers of two). */
+    __device__ __forceinline__ void fetch(const T* src, size_t pos_stride, int t0, int t1, int gap0 = 0, int gap1 = 0) {
+        const int most = min(t1 - t0, 64) - 1, skip = gap0 - t0, to = gap1 - t0;
+        const uint32_t pos_bytes = (uint32_t)(pos_stride * sizeof(T)); /* 64 of them stay within 31 bits */
         const char* from = reinterpret_cast<const char*>(src + (size_t)t0 * pos_stride);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int at = threadIdx.x + NT * u, pg = at / CC, cc = at % CC;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                x[u][i] = *reinterpret_cast<const vec<T, 4>*>(from + (min((uint32_t)(4 * pg + i), most) * pos_bytes + (uint32_t)(4 * sizeof(T)) * cc));
+            for (int i = 0; i < 4; i++) {
+                int t = min(4 * pg + i, most);
+                if (t >= skip && t < to) t = to <= most ? to : max(skip - 1, 0);
+                x[u][i] = *reinterpret_cast<const vec<T, 4>*>(from + ((uint32_t)t * pos_bytes + (uint32_t)(4 * sizeof(T)) * cc));
+            }
         }
     }
     /* the wave's largest magnitude to its slot; finite: of the numbers among them */
@@ -978,12 +983,12 @@ __device__ __forceinline__ void group_part(const attend_args& a, const attend_pa
 template <int HD, typename T>
 constexpr int image_part = (sizeof(T) == 4 ? 2 : 1) * 32 * HD * 2; /* bytes of 32 positions' keys, and of their values behind them */
 
-/* Chunk c (positions 64 c ..) lies in slot c (c < x) or c - y. */
-__device__ __forceinline__ int2 image_slots(const attend_args& a, uint32_t far, uint32_t near) {
+/* Chunk c (positions 64 c ..) lies in slot c (c < x) or c - y; no row sees positions z .. w - 1. */
+__device__ __forceinline__ int4 image_slots(const attend_args& a, uint32_t far, uint32_t near) {
     const int end = min((int)far, a.ctx), least = near ? (int)(0x80000000u - near) : 0;
     const int sink = a.window ? min(a.sinks, end) : 0, from = a.window ? min(max(sink, least - a.window + 1), end) : 0;
     const int n_sink = (sink + 63) >> 6;
-    return make_int2(n_sink, max(n_sink, from >> 6) - n_sink);
+    return make_int4(n_sink, max(n_sink, from >> 6) - n_sink, sink, max(sink, from));
 }
 
 /* Block (key-value head, slot): 64 positions. Bound by bytes: the 5120 positions behind 1024 rows of a 4096 window, 21 MB in
@@ -1019,15 +1024,15 @@ __global__ __launch_bounds__(256) void attend_image_kernel(attend_args a, attend
         near = 0x80000000u - (uint32_t)a.run_pos;
     }
     if (tid < 2) sbad[tid] = 0;
-    const int2 at = image_slots(a, far, near);
+    const int4 at = image_slots(a, far, near);
     if (blockIdx.x == 0 && tid == 0) p.meta[0] = make_int4(at.x, at.y, 0, 0);
     const int end = min((int)far, a.ctx), c = slot < at.x ? slot : slot + at.y;
     if (64 * c >= end) return;
     const T* ks = (const T*)a.k + (size_t)h * a.head_stride + (size_t)seq * a.seq_stride;
     const T* vs = (const T*)a.v + (size_t)h * a.head_stride + (size_t)seq * a.seq_stride;
     share rk, rv;
-    rk.fetch(ks, a.pos_stride, 64 * c, end);
-    rv.fetch(vs, a.pos_stride, 64 * c, end);
+    rk.fetch(ks, a.pos_stride, 64 * c, end, at.z, at.w);
+    rv.fetch(vs, a.pos_stride, 64 * c, end, at.z, at.w);
     rk.publish(smax[0]);
     rv.publish(smax[1]);
     __syncthreads();

@@ -150,6 +150,7 @@ static bool attend(attend_args& a, const float* q, size_t q_stride, float* out, 
     a.out_stride = out_stride ? out_stride : width;
     if (a.q_stride % 4 || a.out_stride % 4 || (a.out_stride < width && a.n > 1) || a.q_stride > EXTENT_MAX / (1 << 20) || a.out_stride > EXTENT_MAX / (1 << 20))
         return fail(err, err_len, "rows %zu and %zu floats apart; a multiple of 4 is needed, the output's at least %zu", a.q_stride, a.out_stride, width);
+    if (q == out && a.q_stride != a.out_stride && a.n > 1) return fail(err, err_len, "out is q, with rows %zu floats apart for %zu", a.out_stride, a.q_stride);
     if (!aligned16(q) || !aligned16(out) || !aligned16(work) || !aligned16(a.rows)) return fail(err, err_len, "q, out, rows and work have to be 16-byte aligned");
     const size_t need = attend_work(a);
     if (work_bytes < need) return fail(err, err_len, "%zu bytes of work; the call needs %zu", work_bytes, need);
