@@ -105,6 +105,26 @@ def test_window_on_every_path(name, window, sinks):
             pair.check(dev, rows, window, sinks)
 
 
+def test_a_window_over_a_long_cache():
+    """A chunk in a cache so long that images of all of it are more than the call takes, at a position where they are not."""
+    with Pair("g4", n_layers=1, n_heads=32, n_kv_heads=16, ctx=20000, seqs=1) as (pair, dev):
+        dev.set_window(4096, 4)
+        rows = [(i % 1000, 7168 + i, 0) for i in range(1024)]
+        dev.rows_step(rows)
+        pair.check(dev, rows, 4096, 4, [0, 700, 1023])
+
+
+def test_a_prefix_near_the_caches_end():
+    """Rows behind a prefix whose power of two lies past the cache."""
+    with Pair("g4") as (pair, dev):
+        dev.kv_fork(2, 650, [5, 0, 7])
+        rows = [(3 + i, 690 + i, s) for i, s in enumerate((2, 5, 0, 7))]
+        dev.rows_step(rows)
+        dev.set_exact_rows(0)
+        dev.rows_step(rows)
+        pair.check(dev, rows, 0, 0)
+
+
 def test_window_taken_away():
     """window 0, or as long as the cache, is the model as it was, bit for bit; a changed window is honoured by graphs made
     before; the persistent step is not taken with one."""

@@ -770,7 +770,7 @@ static hipError_t enqueue_attend(vitna_cuda_model* g, int layer, attn_args a, bo
         t.run = 1;
     } else if (g->rows_prefix) {
         t.share = g->share_dev;
-        t.shared_max = g->rows_prefix;
+        t.shared_max = std::min(g->rows_prefix, g->ctx);
         t.own_max = std::min(g->rows_own, g->ctx);
     }
     return launch_attend(t, g->stream);
@@ -2858,9 +2858,12 @@ static bool ensure_serve(vitna_cuda_model* g, char* err, size_t err_len) {
         size_t most = 0;
         attend_args t = model_attend(g, 0, 1);
         t.window = 0;
-        t.own_max = t.shared_max = g->ctx;
+        t.shared_max = g->ctx;
         for (t.n = 1; t.n <= ROWS_MAX; t.n++)
-            for (int kind = 0; kind < 4; kind++) {
+            for (int i = 0; i < 4 * 32; i++) { /* rows apart, behind a prefix, a prompt's chunk, exact ones; up to every power of two (a shorter chunk may want more: images) */
+                const int kind = i % 4;
+                if (i >= 4 && ATTN_CHUNK << (i / 4 - 1) >= g->ctx) break;
+                t.own_max = (int)std::min<long>((long)ATTN_CHUNK << (i / 4), g->ctx);
                 attend_args x = t;
                 if (kind == 1) x.shared_max = 0;
                 if (kind == 2) { x.shared_max = 0; x.run = 1; }
