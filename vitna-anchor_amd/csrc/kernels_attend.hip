@@ -1322,14 +1322,15 @@ static attend_parts plan(const attend_args& a) {
         return p;
     }
     if (a.shared_max) {
-        /* of groups of few columns two blocks a compute unit, of others one; a tile's groups may need a block each */
+        /* a block a compute unit; a tile's groups may need a block each */
         const long chunks = (a.window ? std::min<long>(a.shared_max, (long)a.window + a.sinks) : a.shared_max) / 64 + 1;
         const bool few = (long)a.n * G <= FEW_CALL;
         p.few = few ? FEW_CALL : FEW_COLUMNS;
-        /* (with twice as many splits the same 40 rows took 65 us for 53, and 32 rows behind 8192 positions 60 for 45) */
+        /* Twice as many splits: 40 rows of 16 key-value heads in groups of eight behind 2048 positions (float32) 52 us for 44,
+           behind 8000 134 for 128 (bfloat16 94 for 112), 32 rows of 4 behind 8192 60 for 45. */
         const long at_once = std::max<long>(1, blocks / ((long)p.tiles * a.n_kv));
         const long groups = std::min(a.n, rows), big = std::min<long>(32 * TILE_COLUMNS / (FEW_COLUMNS + 1), groups); /* a tile's units at most: a row is one at most */
-        p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), few ? 2 * at_once : at_once);
+        p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), at_once);
         p.busy = few ? p.tile : (int)at_once;
         p.few_blocks = (int)std::min<long>(std::max<long>(p.busy, groups), groups * p.tile);
         p.tile_blocks = (int)std::min<long>(std::max<long>(p.busy, big), big * p.tile);
