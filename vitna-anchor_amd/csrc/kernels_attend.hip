@@ -1179,7 +1179,7 @@ __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_own_kernel(attend_ar
 }
 
 /* The prefixes of groups of few columns and the rows' own parts. 40 rows of 16 heads of 128 in groups of eight behind 2048
-   positions (bfloat16): 139 MB in 46-48 us, 3 TB/s; the blocks of a group's prefix are long ones, and its products (16
+   positions (bfloat16): 139 MB in 46-49 us, 3 TB/s; the blocks of a group's prefix are long ones, and its products (16
    columns, half of them used) run beside the loads of the next step. 32 rows' own 256 positions (float32): 11 us. */
 template <int HD, typename T>
 __global__ __launch_bounds__(64 * OWN_WAVES, 2) void attend_columns_kernel(attend_args a, attend_parts p) {

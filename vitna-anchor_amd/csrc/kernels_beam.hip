@@ -57,7 +57,7 @@ static __host__ __device__ size_t beam_sums_bytes(size_t slices) { return (slice
 __device__ __forceinline__ bool beam_before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
 /* Bound by the logits' bytes where they are many: 64 rows of 151936, 39 MB in 14-16 us, 2.4-2.8 TB/s; by the chain of its
-   steps where they are few (4 rows: 7 us). */
+   steps where they are few (4 rows: 9 us, with slices of 16 a lane 7). */
 template <int E, bool VEC>
 __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_args a, int splits) {
     __shared__ float sm[BEAM_WAVES], ss[BEAM_WAVES];
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(64 * BEAM_WAVES) void beam_scan_kernel(beam_select_
 #define PICK_FEW 96    /* and without cutting them first (with 512: 8 beams of 16 kept 24 us for 21, 8 groups of those 26 for 23; with 32: 15 for 13 where 8 are kept) */
 
 /* Latency: a block a group, its slices' sums and candidates (one load each), the bound, the candidates that reach it, their
-   ranks. 9 us for 4 or 8 beams of 151936, 15 for 32 beams of 40000 with 64 kept. */
+   ranks. 5 us for 4 beams of 151936, 9 for 8, 15 for 32 beams of 40000 with 64 kept. */
 __global__ __launch_bounds__(PICK_THREADS) void beam_pick_kernel(beam_select_args a, int splits) {
     __shared__ beam_cand s_cand[PICK_HELD];
     __shared__ double s_score[64], s_log[64]; /* of a beam: its score (-inf: it has no continuations), log of its sum of exponentials */
