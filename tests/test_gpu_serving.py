@@ -375,6 +375,29 @@ def test_large_numbers_that_no_row_sees(dtype, hd, huge, window, sinks):
             check(rows_call(dev, cache, q, rows, window, sinks, 100, 600), want, bound, ("rows", pos0, n))
 
 
+@pytest.mark.parametrize("dtype,heads,kv,hd", [("f32", 16, 1, 64), ("bf16", 2, 2, 128), ("f16", 8, 1, 128)])
+def test_thousands_of_rows(dtype, heads, kv, hd):
+    """Hundreds of tiles of rows, alone, in groups of one to forty and as one run."""
+    n, ctx, seqs = 3001, 3100, 6
+    r = np.random.RandomState(24)
+    with Device() as dev:
+        cache = Cache(dev, dtype, seqs, ctx, kv, hd, seed=25)
+        q = queries(n, heads, hd, 26)
+        some = sorted(set(r.randint(0, n, 40)) | {0, n - 1})
+        rows = [(i % seqs, int(r.randint(-1, 60)), 0, 0) for i in range(n)]
+        want, bound = cache.attend(q[some], [rows[i] for i in some], 20, 2)
+        check(rows_call(dev, cache, q, rows, 20, 2, 60)[some], want, bound, "alone")
+        rows, g = [], 0
+        while len(rows) < n:
+            g += 1
+            rows += [((g + 1 + j) % seqs, 20 + g % 30 + j % 7, g % seqs, 20 + g % 30) for j in range(1 + (g * g) % 40)]
+        rows = rows[:n]
+        want, bound = cache.attend(q[some], [rows[i] for i in some], 0, 0)
+        check(rows_call(dev, cache, q, rows, own_max=8, shared_max=50)[some], want, bound, "groups")
+        want, bound = cache.attend(q[some], [(2, 99 + i, 0, 0) for i in some], 40, 3)
+        check(run_call(dev, cache, q, 2, 99, 40, 3)[some], want, bound, "run")
+
+
 def test_wide_scores_and_a_scale():
     """Scores of thousands: one position takes all the weight; and scores all alike, far below zero."""
     with Device() as dev:
@@ -554,6 +577,16 @@ def test_selection(groups, width, vocab, keep, stride):
             end = vocab // 2
             check_select(select_call(dev, logits, scores, e, end, groups, width, keep, stride),
                          select_want(logits, scores, e, end, groups, width, keep))
+
+
+def test_selection_of_many_groups():
+    r = np.random.RandomState(27)
+    groups, width, vocab, keep = 700, 3, 257, 5
+    logits = (3.0 * r.standard_normal((groups * width, vocab))).astype(np.float32)
+    scores = r.standard_normal(groups * width).astype(np.float32)
+    ended = (r.randint(0, 4, groups * width) == 0).astype(np.uint8)
+    with Device() as dev:
+        check_select(select_call(dev, logits, scores, ended, 9, groups, width, keep), select_want(logits, scores, ended, 9, groups, width, keep))
 
 
 def test_selection_of_equal_values():
