@@ -451,14 +451,6 @@ __device__ __forceinline__ void few_part(const attend_args& a, const attend_part
 
 /* f16 parts, cut: two at once */
 __device__ __forceinline__ uint32_t pack_cut(float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y)); }
-__device__ __forceinline__ float half_lo(uint32_t u) { return (float)__builtin_bit_cast(_Float16, (uint16_t)u); }
-__device__ __forceinline__ float half_hi(uint32_t u) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16)); }
-/* hi and lo of four values times a power of two */
-__device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, float s, uint2& hi, uint2& lo) {
-    hi = make_uint2(pack_cut(x0 * s, x1 * s), pack_cut(x2 * s, x3 * s));
-    lo = make_uint2(pack_cut(fmaf(x0, s, -half_lo(hi.x)), fmaf(x1, s, -half_hi(hi.x))), pack_cut(fmaf(x2, s, -half_lo(hi.y)), fmaf(x3, s, -half_hi(hi.y))));
-}
-
 /* x less a half of h: one instruction (the compiler widens the half first) */
 __device__ __forceinline__ float less_lo(float x, uint32_t h) {
     float r;
@@ -470,10 +462,13 @@ __device__ __forceinline__ float less_hi(float x, uint32_t h) {
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
     return r;
 }
+/* hi and lo of four values, and of four times a power of two */
 __device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, uint2& hi, uint2& lo) {
     hi = make_uint2(pack_cut(x0, x1), pack_cut(x2, x3));
     lo = make_uint2(pack_cut(less_lo(x0, hi.x), less_hi(x1, hi.x)), pack_cut(less_lo(x2, hi.y), less_hi(x3, hi.y)));
 }
+
+__device__ __forceinline__ void cut4(float x0, float x1, float x2, float x3, float s, uint2& hi, uint2& lo) { cut4(x0 * s, x1 * s, x2 * s, x3 * s, hi, lo); }
 
 /* The k of 2^k that brings a magnitude to 2^14 .. 2^15 (0 and numbers near it: as far as 2^k reaches). */
 __device__ __forceinline__ int to_half_range(uint32_t mag) { return min(141 - (int)(mag >> 24), 126); }
