@@ -375,6 +375,23 @@ def test_large_numbers_that_no_row_sees(dtype, hd, huge, window, sinks):
             check(rows_call(dev, cache, q, rows, window, sinks, 100, 600), want, bound, ("rows", pos0, n))
 
 
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2300, 3)])
+def test_groups_behind_long_prefixes(shape, window, sinks):
+    """Groups of one to fifty rows behind prefixes long enough for every way to take them, several in a tile."""
+    dtype, heads, kv, hd, layout = shape
+    with Device() as dev:
+        cache = Cache(dev, dtype, 7, 2600, kv, hd, layout, seed=28)
+        rows = []
+        for g, many in enumerate((5, 5, 1, 6, 18, 2, 2, 9, 50, 1, 13, 8)):
+            base, shared = g % 7, 2500 - 61 * g
+            rows += [((base + 1 + j) % 7, min(2599, shared - 3 + (11 * j) % 80), base, shared) for j in range(many)]
+        q = queries(len(rows), heads, hd, 29)
+        some = list(range(0, len(rows), 7)) + [len(rows) - 1]
+        want, bound = cache.attend(q[some], [rows[i] for i in some], window, sinks)
+        check(rows_call(dev, cache, q, rows, window, sinks, 90, 2500)[some], want, bound)
+
+
 @pytest.mark.parametrize("dtype,heads,kv,hd", [("f32", 16, 1, 64), ("bf16", 2, 2, 128), ("f16", 8, 1, 128)])
 def test_thousands_of_rows(dtype, heads, kv, hd):
     """Hundreds of tiles of rows, alone, in groups of one to forty and as one run."""

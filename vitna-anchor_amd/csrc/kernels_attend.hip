@@ -328,12 +328,13 @@ __device__ __forceinline__ void own_part(const attend_args& a, const attend_part
 
 /* ---- rows that share ---- */
 
-/* A group with so many columns at most goes to few_part, any other to tile_part; a call of FEW_CALL columns or fewer has no
-   other groups. 8 rows of 8 heads a key-value head behind 777 positions (float32): 18 us in few_part, 25 in tile_part;
+/* A group with so many columns at most goes to few_part, any other to tile_part; a call of FEW_CALL columns or fewer, or of
+   FEW_WORK columns times shared positions, has no other groups. 8 rows of 8 heads a key-value head behind 777 positions (float32): 18 us in few_part, 25 in tile_part;
    behind 4096, 24 and 31. Four such groups, 32 rows: behind 777 25 and 30, behind 4096 49 and 43 (bfloat16 54 and 34). Eight
-   groups of 32 columns behind 4096: 51 and 55 (bfloat16 55 and 43). */
+   groups of 32 columns behind 4096: 51 and 55 (bfloat16 55 and 43). Two of 64 behind 160: 14 and 23. */
 #define FEW_COLUMNS 32
 #define FEW_CALL 64
+#define FEW_WORK (1L << 18)
 
 /* A tile: 32 columns each of TILE_COLUMNS waves; for tile_part of heads of 128 two waves take the same columns, each half of
    a chunk's positions. */
@@ -393,7 +394,7 @@ __device__ __forceinline__ group_span group_seen(const attend_args& a, const att
 
 /* How a tile's blocks take its units: block y takes unit y mod units, part y / units of its positions (there are blocks for
    every unit). A unit's parts are the first of the tile's p.tile splits, the others get an empty part of its columns.
-   (Blocks that each took their part of unit after unit had 36 rows in groups of two behind 426 positions in 68 us; so 27.) */
+   (Blocks that each took their part of unit after unit had 36 rows in groups of two behind 426 positions in 68 us; so 21.) */
 struct unit_share {
     int units, y, parts;
     __device__ __forceinline__ unit_share(int units_, int busy, int y_, int splits) : units(units_), y(y_), parts(min(max(busy / units_, 1), splits)) {}
@@ -1319,16 +1320,17 @@ static attend_parts plan(const attend_args& a) {
     if (a.shared_max) {
         /* a block a compute unit; a tile's groups may need a block each */
         const long chunks = (a.window ? std::min<long>(a.shared_max, (long)a.window + a.sinks) : a.shared_max) / 64 + 1;
-        const bool few = (long)a.n * G <= FEW_CALL;
-        p.few = few ? FEW_CALL : FEW_COLUMNS;
+        const long columns = (long)a.n * G;
+        const bool few = columns <= FEW_CALL || columns * std::min(chunks * 64, (long)a.shared_max) <= FEW_WORK;
+        p.few = few ? 32 * TILE_COLUMNS : FEW_COLUMNS;
         /* Twice as many splits: 40 rows of 16 key-value heads in groups of eight behind 2048 positions (float32) 52 us for 44,
            behind 8000 134 for 128 (bfloat16 94 for 112), 32 rows of 4 behind 8192 60 for 45. */
         const long at_once = std::max<long>(1, blocks / ((long)p.tiles * a.n_kv));
         const long groups = std::min(a.n, rows), big = std::min<long>(32 * TILE_COLUMNS / (FEW_COLUMNS + 1), groups); /* a tile's units at most: a row is one at most */
-        p.tile = (int)std::min<long>(std::min<long>(few ? 2 * chunks : chunks, 64), at_once);
-        p.busy = few ? p.tile : (int)at_once;
+        p.tile = (int)std::min<long>(std::min<long>(chunks, 64), at_once);
+        p.busy = (int)at_once;
         p.few_blocks = (int)std::min<long>(std::max<long>(p.busy, groups), groups * p.tile);
-        p.tile_blocks = (int)std::min<long>(std::max<long>(p.busy, big), big * p.tile);
+        p.tile_blocks = few ? 0 : (int)std::min<long>(std::max<long>(p.busy, big), big * p.tile);
     }
     p.own = (int)std::min<long>(std::min<long>((seen + 16 * OWN_WAVES - 1) / (16 * OWN_WAVES), ATTEND_SPLITS_MAX), std::max<long>(1, 1024 / ((long)a.n * a.n_kv)));
     if (a.splits) p.own = std::min(a.splits, ATTEND_SPLITS_MAX);
@@ -1363,7 +1365,7 @@ static hipError_t launch(const attend_args& a, const attend_parts& p, hipStream_
         attend_tile_kernel<HD, T, true><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else if (p.tile) {
         attend_columns_kernel<HD, T><<<heads * ((unsigned)p.tiles * p.few_blocks + (unsigned)a.n * p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
-        if ((long)a.n * (a.n_heads / a.n_kv) > p.few) attend_tile_kernel<HD, T, false><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
+        if (p.tile_blocks) attend_tile_kernel<HD, T, false><<<tile_blocks, 64 * NW, 0, s>>>(a, p);
     } else {
         attend_own_kernel<HD, T><<<dim3(a.n * heads, p.own), 64 * OWN_WAVES, 0, s>>>(a, p);
     }
